@@ -8,7 +8,9 @@ gfx950 reached through the C ABI in ``include/gn2v.h``; there is no CPU executio
 from . import _lib
 from .embedding_transformers import (EdgeLabelPredictionTransformer, EdgePredictionTransformer,
                                      EdgeTransformer, GraphTransformer,
-                                     NodeLabelPredictionTransformer, NodeTransformer)
+                                     NodeLabelPredictionTransformer, NodeTransformer,
+                                     QuantizedTable, TypePlan, adapted_projection,
+                                     edge_embedding, typed_projection)
 from .embedders import (DeepWalkCBOWEnsmallen, DeepWalkGloVeEnsmallen, DeepWalkSkipGramEnsmallen,
                         Node2VecCBOWEnsmallen, Node2VecGloVeEnsmallen, Node2VecSkipGramEnsmallen,
                         WalkletsCBOWEnsmallen, WalkletsGloVeEnsmallen,
@@ -30,5 +32,6 @@ __all__ = [
     "get_models_dataframe", "get_available_models_for_node_embedding", "normalize_kwargs",
     "Node2VecSequence", "EdgeTransformer", "NodeTransformer", "GraphTransformer",
     "EdgePredictionTransformer", "EdgeLabelPredictionTransformer",
-    "NodeLabelPredictionTransformer",
+    "NodeLabelPredictionTransformer", "edge_embedding", "QuantizedTable", "TypePlan",
+    "typed_projection", "adapted_projection",
 ]

@@ -11,7 +11,7 @@ import subprocess
 
 _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libgn2v.so")
-_UNITS = ["gn2v_api.hip", "gn2v_block_api.hip", "gn2v_rccl.hip"]  # translation units of libgn2v.so
+_UNITS = ["gn2v_api.hip", "gn2v_block_api.hip", "gn2v_rccl.hip", "gn2v_typed_api.hip"]  # translation units of libgn2v.so
 _HEADER = os.path.join(os.path.dirname(_CSRC), "..", "include", "gn2v.h")
 _HEADER_EXPERIMENTAL = os.path.join(os.path.dirname(_CSRC), "..", "include", "gn2v_experimental.h")
 _HEADER_INTERNAL = os.path.join(os.path.dirname(_CSRC), "..", "include", "gn2v_internal.h")
@@ -56,6 +56,11 @@ INTERNAL_EXPORTS = [
     "gn2v_block_extract", "gn2v_block_cell_offsets", "gn2v_block_step", "gn2v_block_round",
     "gn2v_block_auto_plan", "gn2v_block_auto_plan_graph", "gn2v_block_round_plan",
     "gn2v_graph_xcds", "gn2v_graph_reserve_cus", "gn2v_touch_rows",
+    # the operators on rows of embedding tables (typed_projection, adapted_projection,
+    # QuantizedTable)
+    "gn2v_type_plan_words", "gn2v_type_plan", "gn2v_typed_product", "gn2v_adapted_product",
+    "gn2v_few_rows_product", "gn2v_typed_gradient_temp", "gn2v_typed_gradient",
+    "gn2v_table_write", "gn2v_table_read", "gn2v_table_edge_embedding",
 ]
 EXPORTS = BOUNDARY_EXPORTS + INTERNAL_EXPORTS
 # include/gn2v_rccl.h: a gn2v_comm filled with RCCL calls, for hosts without Python (RCCL is
@@ -207,6 +212,76 @@ BLOCK_HOT_MAX = 192      # GN2V_BLOCK_HOT_MAX
 BLOCK_HOT_DEFAULT = 192  # GN2V_BLOCK_HOT_DEFAULT
 
 
+MAX_TYPES = 32768            # GN2V_MAX_TYPES
+MAX_RANK = 64                # GN2V_MAX_RANK
+FEW_ROWS_DEPTH = 4096        # GN2V_FEW_ROWS_DEPTH
+TABLE_FEW_ENTRIES = 1024     # GN2V_TABLE_FEW_ENTRIES
+
+
+class Weights(C.Structure):
+    """gn2v_weights (include/gn2v_internal.h)."""
+    _fields_ = [("d_data", C.c_void_p), ("type_stride", C.c_int64), ("inner", C.c_int64),
+                ("outer", C.c_int64)]
+
+
+class ProductIO(C.Structure):
+    """gn2v_product_io (include/gn2v_internal.h)."""
+    _fields_ = [
+        ("dtype", C.c_uint32),
+        ("n_types", C.c_uint32),
+        ("rows", C.c_uint64),
+        ("inputs", C.c_uint32),
+        ("outputs", C.c_uint32),
+        ("d_x", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("weight", Weights),
+        ("d_bias", C.c_void_p),
+        ("bias_stride", C.c_int64),
+        ("d_y", C.c_void_p),
+        ("ldy", C.c_int64),
+        ("d_plan", C.c_void_p),
+        ("d_types", C.c_void_p),
+        ("type_bytes", C.c_uint32),
+        ("rank", C.c_uint32),
+        ("scale", C.c_float),
+        ("low_rank_rows", C.c_uint32),
+        ("down", Weights),
+        ("up", Weights),
+        ("d_low", C.c_void_p),
+    ]
+
+
+class GradientIO(C.Structure):
+    """gn2v_gradient_io (include/gn2v_internal.h)."""
+    _fields_ = [
+        ("dtype", C.c_uint32),
+        ("n_types", C.c_uint32),
+        ("rows", C.c_uint64),
+        ("inputs", C.c_uint32),
+        ("outputs", C.c_uint32),
+        ("d_x", C.c_void_p),
+        ("d_dy", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("ldy", C.c_int64),
+        ("x_low", C.c_uint32),
+        ("y_low", C.c_uint32),
+        ("shared", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("d_plan", C.c_void_p),
+        ("d_dw", C.c_void_p),
+        ("d_db", C.c_void_p),
+        ("d_temp", C.c_void_p),
+        ("temp_bytes", C.c_uint64),
+    ]
+
+
+class Table8(C.Structure):
+    """gn2v_table8 (include/gn2v_internal.h)."""
+    _fields_ = [("d_codes", C.c_void_p), ("d_scales", C.c_void_p), ("rows", C.c_uint64),
+                ("d", C.c_uint32), ("stride", C.c_uint32), ("group", C.c_uint32),
+                ("code", C.c_uint32)]
+
+
 class Stats(C.Structure):
     _fields_ = [
         ("pairs", C.c_uint64),
@@ -333,6 +408,16 @@ def lib():
                                    u64, C.POINTER(Comm), vp, vp, C.POINTER(Stats), vp]
     L.gn2v_train_blocks.argtypes = [vp, C.POINTER(WalkParams), C.POINTER(TrainParams), u64, u64,
                                     u64, u32, vp, vp, C.POINTER(Stats), vp]
+    L.gn2v_type_plan_words.argtypes = [u64, u32, C.POINTER(u64), C.POINTER(u64)]
+    L.gn2v_type_plan.argtypes = [vp, u32, u64, u32, vp, vp, vp]
+    for product in ("gn2v_typed_product", "gn2v_adapted_product", "gn2v_few_rows_product"):
+        getattr(L, product).argtypes = [C.POINTER(ProductIO), vp]
+    L.gn2v_typed_gradient_temp.argtypes = [C.POINTER(GradientIO), C.POINTER(u64)]
+    L.gn2v_typed_gradient.argtypes = [C.POINTER(GradientIO), vp]
+    L.gn2v_table_write.argtypes = [C.POINTER(Table8), vp, u32, C.c_int64, vp, u32, u64, vp, vp]
+    L.gn2v_table_read.argtypes = [C.POINTER(Table8), vp, u32, u64, vp, u32, C.c_int64, vp]
+    L.gn2v_table_edge_embedding.argtypes = [C.POINTER(Table8), C.POINTER(Table8), vp, vp, u32, u64,
+                                            u32, vp, C.c_int64, vp]
     L.gn2v_graph_release_buffers.argtypes = [vp]
     L.gn2v_graph_walk_accel.argtypes = [vp]
     L.gn2v_stats_reset.argtypes = [vp, vp]

@@ -1,0 +1,570 @@
+// libgn2v.so -- the operators on rows of embedding tables declared at the end of gn2v_internal.h:
+// typed and adapted products, their gradients, tables in 8 bits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "../../include/gn2v_internal.h"
+#include "handle.h"
+#include "quantized_kernels.h"
+#include "typed_kernels.h"
+
+using namespace gn2v_host;
+
+namespace {
+
+constexpr uint64_t kMaxRows = (1ull << 31) - (1ull << 20);  // positions are int32
+
+// the plan's words and the stripes its rows are counted in
+struct PlanSizes {
+    uint64_t tile_bound, words, temp;
+    uint32_t stripes, stripe;
+};
+
+PlanSizes plan_sizes(uint64_t rows, uint32_t types) {
+    PlanSizes s;
+    s.tile_bound = std::min<uint64_t>(rows, (rows + 63) / 64 + std::min<uint64_t>(types + 1ull, rows));
+    s.words = (2 * rows + types + 2 + 1) / 2 * 2 + 2 * s.tile_bound;
+    // one wave each: 512 rows at least, and at most 4 M counters in all
+    uint64_t stripes = std::min<uint64_t>((rows + 511) / 512, 4096);
+    stripes = std::max<uint64_t>(1, std::min<uint64_t>(stripes, (1ull << 22) / (types + 1)));
+    s.stripe = (uint32_t)(((rows + stripes - 1) / stripes + 63) / 64 * 64);
+    s.stripes = s.stripe ? (uint32_t)((rows + s.stripe - 1) / s.stripe) : 0;
+    s.temp = rows <= gn2v::kSmallPlan ? 0 : (uint64_t)s.stripes * (types + 1) + types + 1;
+    return s;
+}
+
+gn2v::PlanView plan_view(const int32_t *d_plan, uint64_t rows, uint32_t types) {
+    gn2v::PlanView v{};
+    v.rows = (uint32_t)rows;
+    v.types = types;
+    if (!d_plan) return v;
+    int *p = const_cast<int32_t *>(d_plan);
+    v.order = p;
+    v.row_types = p + rows;
+    v.offsets = p + 2 * rows;
+    v.tile_bound = (uint32_t)plan_sizes(rows, types).tile_bound;
+    v.tiles = reinterpret_cast<int2 *>(p + (2 * rows + types + 2 + 1) / 2 * 2);
+    return v;
+}
+
+int check_plan(uint64_t rows, uint32_t types) {
+    if (rows > kMaxRows) return fail("too many rows: at most 2^31 - 2^20");
+    if (types < 1 || types > GN2V_MAX_TYPES) return fail("need 1 <= n_types <= 32768");
+    return 0;
+}
+
+uint32_t size_of(uint32_t dtype) { return dtype == GN2V_F32 ? 4 : 2; }
+
+// the largest power of two up to 16 bytes that divides a row's address, whichever row
+int alignment(const void *base, int64_t stride_elements, uint32_t size) {
+    const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride_elements * (int64_t)size) | 16u;
+    return (int)(bits & (~bits + 1));
+}
+
+template <typename I>
+void launch_plan(const I *types, const gn2v::PlanView &v, int32_t *temp, hipStream_t s) {
+    if (v.rows <= gn2v::kSmallPlan) {
+        hipLaunchKernelGGL((gn2v::plan_small_kernel<I>), dim3(1), dim3(gn2v::kSmallPlan), 0, s, types, v);
+        return;
+    }
+    const PlanSizes z = plan_sizes(v.rows, v.types);
+    const size_t lds = (v.types + 1) * sizeof(int);
+    if (lds > 65536) {  // more than 16 383 types: the counters need more than the default limit
+        (void)hipFuncSetAttribute((const void *)gn2v::plan_count_kernel<I>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        (void)hipFuncSetAttribute((const void *)gn2v::plan_place_kernel<I>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    }
+    int *counts = temp, *totals = temp + (uint64_t)z.stripes * (v.types + 1);
+    hipLaunchKernelGGL((gn2v::plan_count_kernel<I>), dim3(z.stripes), dim3(64), lds, s, types, v.rows,
+                       v.types, z.stripe, z.stripes, counts);
+    hipLaunchKernelGGL(gn2v::plan_scan_kernel, dim3(v.types + 1), dim3(256), 0, s, counts, z.stripes,
+                       totals);
+    hipLaunchKernelGGL(gn2v::plan_pieces_kernel, dim3(1), dim3(1024), 0, s, totals, v.offsets,
+                       v.types + 1, (uint32_t)gn2v::kTileRows, v.tile_bound, v.tiles, (int *)nullptr);
+    int bits = 0;
+    while (v.types >> bits) ++bits;
+    hipLaunchKernelGGL((gn2v::plan_place_kernel<I>), dim3(z.stripes), dim3(64), lds, s, types, v,
+                       z.stripe, z.stripes, counts, bits);
+}
+
+int check_product(const gn2v_product_io *io) {
+    if (!io) return fail("NULL io");
+    if (io->dtype != GN2V_F32 && io->dtype != GN2V_BF16) return fail("unknown dtype");
+    if (check_plan(io->rows, io->n_types)) return 1;
+    if (io->inputs == 0 || io->outputs == 0 || io->inputs > (1u << 20) || io->outputs > (1u << 20))
+        return fail("need 1 <= inputs, outputs <= 2^20");
+    if (io->rank > GN2V_MAX_RANK) return fail("rank must be at most 64");
+    if (io->ldx < (int64_t)io->inputs || io->ldy < (int64_t)io->outputs)
+        return fail("row strides must hold a row");
+    if (io->rows && (!io->d_x || !io->weight.d_data || !io->d_y)) return fail("NULL pointer");
+    if (io->weight.inner != 1 && io->weight.outer != 1)
+        return fail("one of the weights' two strides must be 1");
+    return 0;
+}
+
+gn2v::WeightView view_of(const gn2v_weights &w, uint32_t size) {
+    gn2v::WeightView v{w.d_data, w.type_stride, w.inner, w.outer, 0};
+    const int64_t row = w.outer == 1 ? w.inner : w.outer;
+    v.align = std::min(alignment(w.d_data, row, size), alignment(nullptr, w.type_stride, size));
+    return v;
+}
+
+gn2v::ProductArgs product_args(const gn2v_product_io *io) {
+    const uint32_t size = size_of(io->dtype);
+    gn2v::ProductArgs a{};
+    a.x = io->d_x;
+    a.ldx = io->ldx;
+    a.x_align = alignment(io->d_x, io->ldx, size);
+    a.w = view_of(io->weight, size);
+    a.bias = io->d_bias;
+    a.bias_type = io->bias_stride;
+    a.y = io->d_y;
+    a.ldy = io->ldy;
+    a.sorted = io->low_rank_rows != 0;
+    const uint32_t out = a.sorted ? 4 : size;
+    a.y_vec = alignment(io->d_y, io->ldy, out) >= (int)(4 * out);
+    a.scale = io->scale;
+    a.plan = plan_view(io->d_plan, io->rows, io->n_types);
+    a.K = (int)io->inputs;
+    a.N = (int)io->outputs;
+    return a;
+}
+
+template <typename T, int BN, bool WT, bool ADAPT>
+void launch_product_kernel(const gn2v::ProductArgs &a, hipStream_t s) {
+    const uint64_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : a.plan.tile_bound;
+    const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8 * ((a.N + BN - 1) / BN));
+    hipLaunchKernelGGL((gn2v::product_kernel<T, BN, WT, ADAPT>), dim3(blocks), dim3(256), 0, s, a);
+}
+
+template <typename T, bool WT, bool ADAPT>
+void launch_product_bn(const gn2v::ProductArgs &a, hipStream_t s) {
+    if (a.N <= 32)
+        launch_product_kernel<T, 32, WT, ADAPT>(a, s);
+    else if (a.N <= 64)
+        launch_product_kernel<T, 64, WT, ADAPT>(a, s);
+    else
+        launch_product_kernel<T, 128, WT, ADAPT>(a, s);
+}
+
+template <bool ADAPT>
+int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, hipStream_t s) {
+    const uint64_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : a.plan.tile_bound;
+    if (((tiles + 7) / 8 * 8) * ((a.N + 31) / 32) > 0x7FFFFFFFull) return fail("too many tiles for one launch");
+    const bool wt = a.w.outer != 1;
+    if (dtype == GN2V_F32)
+        wt ? launch_product_bn<float, true, ADAPT>(a, s) : launch_product_bn<float, false, ADAPT>(a, s);
+    else
+        wt ? launch_product_bn<__bf16, true, ADAPT>(a, s) : launch_product_bn<__bf16, false, ADAPT>(a, s);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+// how the rows of a gradient are cut: about 1024 workgroups over the chunks and blocks of dw, pieces
+// of 128 rows at least, and no more than 256 MB of partial sums beside the one per type
+struct GradSizes {
+    uint32_t bm, bn, chunk_rows;
+    uint64_t chunks, stride, list_words, bytes;
+};
+
+GradSizes grad_sizes(const gn2v_gradient_io *io) {
+    GradSizes g;
+    g.bm = io->inputs <= 32 ? 32 : io->inputs <= 64 ? 64 : 128;
+    g.bn = io->outputs <= 32 ? 32 : io->outputs <= 64 ? 64 : 128;
+    const uint64_t blocks = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm) * ((io->outputs + g.bn - 1) / g.bn);
+    g.stride = (((uint64_t)io->inputs + 1) * io->outputs + 3) / 4 * 4;
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>((1024 + blocks - 1) / blocks, (64ull << 20) / g.stride));
+    uint64_t rows = (io->rows + most - 1) / most;
+    rows = std::max<uint64_t>(128, (rows + 63) / 64 * 64);
+    g.chunk_rows = (uint32_t)rows;
+    g.chunks = (io->rows + rows - 1) / rows;
+    g.list_words = 0;
+    if (!io->shared) {
+        g.chunks += std::min<uint64_t>(io->n_types, io->rows);
+        g.list_words = (2 * g.chunks + io->n_types + 1 + 3) / 4 * 4;
+    }
+    g.bytes = g.list_words * 4 + g.chunks * g.stride * 4;
+    return g;
+}
+
+int check_gradient(const gn2v_gradient_io *io) {
+    if (!io) return fail("NULL io");
+    if (io->dtype != GN2V_F32 && io->dtype != GN2V_BF16) return fail("unknown dtype");
+    if (check_plan(io->rows, io->n_types)) return 1;
+    if (io->outputs == 0 || io->inputs > (1u << 20) || io->outputs > (1u << 20))
+        return fail("need inputs <= 2^20, 1 <= outputs <= 2^20");
+    if (io->x_low && io->y_low) return fail("at most one operand is low-rank rows");
+    if ((io->x_low && io->inputs > GN2V_MAX_RANK) || (io->y_low && io->outputs > GN2V_MAX_RANK))
+        return fail("low-rank rows are at most 64 wide");
+    return 0;
+}
+
+template <typename T, int MI, int NI>
+void launch_grad_low(const gn2v_gradient_io *io, const gn2v::GradArgs &a, unsigned blocks, hipStream_t s) {
+    // low-rank rows are at most 64 wide (check_gradient)
+    if constexpr (MI <= 2)
+        if (io->x_low) {
+            hipLaunchKernelGGL((gn2v::grad_kernel<T, MI, NI, true, false>), dim3(blocks), dim3(256), 0, s, a);
+            return;
+        }
+    if constexpr (NI <= 2)
+        if (io->y_low) {
+            hipLaunchKernelGGL((gn2v::grad_kernel<T, MI, NI, false, true>), dim3(blocks), dim3(256), 0, s, a);
+            return;
+        }
+    hipLaunchKernelGGL((gn2v::grad_kernel<T, MI, NI, false, false>), dim3(blocks), dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_grad(const gn2v_gradient_io *io, const GradSizes &g, const gn2v::GradArgs &a, unsigned blocks,
+                 hipStream_t s) {
+#define GN2V_GRAD(BM, BN) \
+    if (g.bm == BM && g.bn == BN) launch_grad_low<T, BM / 32, BN / 32>(io, a, blocks, s)
+    GN2V_GRAD(32, 32);
+    GN2V_GRAD(32, 64);
+    GN2V_GRAD(32, 128);
+    GN2V_GRAD(64, 32);
+    GN2V_GRAD(64, 64);
+    GN2V_GRAD(64, 128);
+    GN2V_GRAD(128, 32);
+    GN2V_GRAD(128, 64);
+    GN2V_GRAD(128, 128);
+#undef GN2V_GRAD
+}
+
+int check_table(const gn2v_table8 *t) {
+    if (!t) return fail("NULL table");
+    if (t->code != GN2V_INT8 && t->code != GN2V_E4M3) return fail("unknown code type");
+    if (t->group != 16 && t->group != 32 && t->group != 64 && t->group != 128)
+        return fail("group must be 16, 32, 64 or 128");
+    if (t->d == 0 || t->d > (1u << 20) || t->stride < t->d || (t->stride & 15))
+        return fail("need 0 < d <= stride, stride % 16 == 0, d <= 2^20");
+    if (t->rows && (!t->d_codes || !t->d_scales)) return fail("NULL pointer");
+    if ((uintptr_t)t->d_codes & 15) return fail("codes must be 16-byte aligned");
+    return 0;
+}
+
+gn2v::TableView table_view(const gn2v_table8 *t) {
+    gn2v::TableView v;
+    v.codes = (uint8_t *)t->d_codes;
+    v.scales = t->d_scales;
+    v.rows = t->rows;
+    v.d = t->d;
+    v.stride = t->stride;
+    v.group_shift = t->group == 16 ? 4 : t->group == 32 ? 5 : t->group == 64 ? 6 : 7;
+    v.groups = (t->d + t->group - 1) / t->group;
+    return v;
+}
+
+// lanes per row: eight columns each, a power of two, a wave at most
+int lanes_shift(uint32_t d) {
+    int shift = 0;
+    while (shift < 6 && (8u << shift) < d) ++shift;
+    return shift;
+}
+
+unsigned row_blocks(uint64_t n, int shift) {
+    const uint64_t per = 256u >> shift;
+    return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((n + per - 1) / per, 256 * 32));
+}
+
+int check_ids(const void *ids, uint32_t id_bytes) {
+    if (ids && id_bytes != 4 && id_bytes != 8) return fail("id_bytes must be 4 or 8");
+    return 0;
+}
+
+template <typename T>
+void launch_write(const gn2v_table8 *t, const gn2v::TableView &v, const void *values, int64_t ldv,
+                  const void *ids, uint32_t id_bytes, uint64_t n, const int32_t *owner, hipStream_t s) {
+    const int shift = lanes_shift(t->d), align = alignment(values, ldv, sizeof(T));
+    const unsigned blocks = row_blocks(n, shift);
+    if (t->code == GN2V_INT8)
+        hipLaunchKernelGGL((gn2v::table_write_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v,
+                           (const T *)values, ldv, align, ids, (int)id_bytes, n, owner, shift);
+    else
+        hipLaunchKernelGGL((gn2v::table_write_kernel<T, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, v,
+                           (const T *)values, ldv, align, ids, (int)id_bytes, n, owner, shift);
+}
+
+template <typename T>
+void launch_read(const gn2v_table8 *t, const gn2v::TableView &v, const void *ids, uint32_t id_bytes,
+                 uint64_t n, void *out, int64_t ldo, hipStream_t s) {
+    const int shift = lanes_shift(t->d), vec = alignment(out, ldo, sizeof(T)) == 16;
+    const unsigned blocks = row_blocks(n, shift);
+    if (t->code == GN2V_INT8)
+        hipLaunchKernelGGL((gn2v::table_read_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v, ids,
+                           (int)id_bytes, n, (T *)out, ldo, vec, shift);
+    else
+        hipLaunchKernelGGL((gn2v::table_read_kernel<T, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, v, ids,
+                           (int)id_bytes, n, (T *)out, ldo, vec, shift);
+}
+
+template <uint32_t METHOD>
+void launch_edges(uint32_t code, const gn2v::TableView &a, const gn2v::TableView &b, const void *u,
+                  const void *w, uint32_t id_bytes, uint64_t n, float *out, int64_t ldo, hipStream_t s) {
+    const int shift = lanes_shift(a.d);
+    const int vec = alignment(out, ldo, 4) == 16 && (METHOD != gn2v::kConcatenate || (a.d & 3) == 0);
+    const unsigned blocks = row_blocks(n, shift);
+    if (code == GN2V_INT8)
+        hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, a,
+                           b, u, w, (int)id_bytes, n, out, ldo, vec, shift);
+    else
+        hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, a,
+                           b, u, w, (int)id_bytes, n, out, ldo, vec, shift);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gn2v_type_plan_words(uint64_t rows, uint32_t n_types, uint64_t *plan_words, uint64_t *temp_words) {
+    if (!plan_words || !temp_words) return fail("NULL pointer");
+    if (check_plan(rows, n_types)) return 1;
+    const PlanSizes s = plan_sizes(rows, n_types);
+    *plan_words = s.words;
+    *temp_words = s.temp;
+    return 0;
+}
+
+int gn2v_type_plan(const void *d_types, uint32_t type_bytes, uint64_t rows, uint32_t n_types,
+                   int32_t *d_plan, int32_t *d_temp, void *stream) {
+    if (check_plan(rows, n_types)) return 1;
+    if (type_bytes != 4 && type_bytes != 8) return fail("type_bytes must be 4 or 8");
+    if (!d_plan || (rows && !d_types) || (plan_sizes(rows, n_types).temp && !d_temp))
+        return fail("NULL pointer");
+    DeviceGuard guard(DeviceGuard::of_pointer(d_plan));
+    const gn2v::PlanView v = plan_view(d_plan, rows, n_types);
+    if (type_bytes == 8)
+        launch_plan((const int64_t *)d_types, v, d_temp, (hipStream_t)stream);
+    else
+        launch_plan((const int32_t *)d_types, v, d_temp, (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_typed_product(const gn2v_product_io *io, void *stream) {
+    if (check_product(io)) return 1;
+    if (io->rows == 0) return 0;
+    if (!io->d_plan) return fail("NULL plan");
+    DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
+    return launch_product<false>(io->dtype, product_args(io), (hipStream_t)stream);
+}
+
+int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
+    if (check_product(io)) return 1;
+    if (io->rank == 0) return fail("need a rank of at least 1");
+    if (io->low_rank_rows) return fail("low_rank_rows belongs to gn2v_typed_product");
+    if (io->rows == 0) return 0;
+    if (!io->d_plan || !io->d_low || !io->up.d_data) return fail("NULL pointer");
+    if ((io->weight.outer == 1) != (io->up.outer == 1) && io->rank > 1)
+        return fail("weight and up must be laid out alike");
+    DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
+    gn2v::ProductArgs a = product_args(io);
+    a.scale = 1.f;  // the low-rank rows hold it
+    a.bias_type = 0;
+    a.low = io->d_low;
+    a.rank = (int)io->rank;
+    a.up = view_of(io->up, size_of(io->dtype));
+    return launch_product<true>(io->dtype, a, (hipStream_t)stream);
+}
+
+int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
+    if (check_product(io)) return 1;
+    if (io->inputs > GN2V_FEW_ROWS_DEPTH || io->rows > 65535)
+        return fail("need inputs <= 4096 and rows <= 65535");
+    if (io->low_rank_rows) return fail("low_rank_rows belongs to gn2v_typed_product");
+    if (io->weight.outer != 1 || (io->rank && (io->down.outer != 1 || io->up.outer != 1)))
+        return fail("weights must have contiguous rows");
+    if (io->rows == 0) return 0;
+    if (!io->d_plan && (!io->d_types || (io->type_bytes != 4 && io->type_bytes != 8)))
+        return fail("need a plan, or int32 / int64 types");
+    if (io->rank && (!io->down.d_data || !io->up.d_data)) return fail("NULL pointer");
+    DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
+    const uint32_t size = size_of(io->dtype);
+    gn2v::FewArgs a{};
+    a.x = io->d_x;
+    a.ldx = io->ldx;
+    a.w = view_of(io->weight, size);
+    a.bias = io->d_bias;
+    a.bias_type = io->bias_stride;
+    a.y = io->d_y;
+    a.ldy = io->ldy;
+    a.types = io->d_plan ? nullptr : io->d_types;
+    a.type_bytes = (int)io->type_bytes;
+    a.plan = plan_view(io->d_plan, io->rows, io->n_types);
+    a.K = (int)io->inputs;
+    a.N = (int)io->outputs;
+    a.rank = (int)io->rank;
+    a.scale = io->scale;
+    const dim3 grid((io->outputs + 63) / 64, (unsigned)io->rows);
+    hipStream_t s = (hipStream_t)stream;
+    if (io->rank) {
+        a.down = view_of(io->down, size);
+        a.up = view_of(io->up, size);
+        if (io->dtype == GN2V_F32)
+            hipLaunchKernelGGL((gn2v::few_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((gn2v::few_rows_kernel<__bf16, true>), grid, dim3(256), 0, s, a);
+    } else if (io->dtype == GN2V_F32) {
+        hipLaunchKernelGGL((gn2v::few_rows_kernel<float, false>), grid, dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((gn2v::few_rows_kernel<__bf16, false>), grid, dim3(256), 0, s, a);
+    }
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_typed_gradient_temp(const gn2v_gradient_io *io, uint64_t *temp_bytes) {
+    if (!temp_bytes) return fail("NULL pointer");
+    if (check_gradient(io)) return 1;
+    *temp_bytes = grad_sizes(io).bytes;
+    return 0;
+}
+
+int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
+    if (check_gradient(io)) return 1;
+    if ((io->inputs && !io->d_dw) || (!io->inputs && !io->d_db)) return fail("NULL gradient");
+    if (io->rows && (!io->d_dy || (io->inputs && !io->d_x))) return fail("NULL pointer");
+    if (io->rows && !io->d_plan && (!io->shared || io->x_low || io->y_low)) return fail("NULL plan");
+    if (io->ldx < (int64_t)io->inputs || io->ldy < (int64_t)io->outputs)
+        return fail("row strides must hold a row");
+    const GradSizes g = grad_sizes(io);
+    if (io->temp_bytes < g.bytes || (g.bytes && !io->d_temp)) return fail("d_temp is too small");
+    const uint64_t kb = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm), nb = (io->outputs + g.bn - 1) / g.bn;
+    const uint64_t blocks = (g.chunks + 7) / 8 * 8 * kb * nb;
+    const uint32_t types = io->shared ? 1 : io->n_types;
+    const uint64_t joins = types * ((g.stride + 255) / 256);
+    if (blocks > 0x7FFFFFFFull || joins > 0x7FFFFFFFull) return fail("too many blocks for one launch");
+    DeviceGuard guard(DeviceGuard::of_pointer(io->d_dw ? io->d_dw : io->d_db));
+    hipStream_t s = (hipStream_t)stream;
+    const uint32_t size = size_of(io->dtype);
+    gn2v::GradArgs a{};
+    a.x = io->d_x;
+    a.dy = io->d_dy;
+    a.ldx = io->ldx;
+    a.ldy = io->ldy;
+    a.x_align = alignment(io->d_x, io->ldx, io->x_low ? 4 : size);
+    a.y_align = alignment(io->d_dy, io->ldy, io->y_low ? 4 : size);
+    const gn2v::PlanView v = plan_view(io->d_plan, io->rows, io->n_types);
+    a.rows = (uint32_t)io->rows;
+    a.types = types;
+    a.chunk_rows = g.chunk_rows;
+    a.chunk_bound = (uint32_t)g.chunks;
+    a.K = (int)io->inputs;
+    a.N = (int)io->outputs;
+    a.stride = (int64_t)g.stride;
+    a.dw = io->d_dw;
+    a.db = io->d_db;
+    a.partial = (float *)((char *)io->d_temp + g.list_words * 4);
+    if (!io->shared && io->rows) {
+        int2 *chunks = (int2 *)io->d_temp;
+        int *first = (int *)(chunks + g.chunks);
+        hipLaunchKernelGGL(gn2v::plan_pieces_kernel, dim3(1), dim3(1024), 0, s, (const int *)nullptr,
+                           v.offsets, io->n_types, g.chunk_rows, (uint32_t)g.chunks, chunks, first);
+        a.order = v.order;
+        a.offsets = v.offsets;
+        a.chunks = chunks;
+        a.first = first;
+    }
+    if (io->rows) {
+        if (io->dtype == GN2V_F32)
+            launch_grad<float>(io, g, a, (unsigned)blocks, s);
+        else
+            launch_grad<__bf16>(io, g, a, (unsigned)blocks, s);
+        HIP_TRY(hipGetLastError());
+    }
+    if (io->dtype == GN2V_F32)
+        hipLaunchKernelGGL((gn2v::grad_join_kernel<float>), dim3((unsigned)joins), dim3(1024), 0, s, a);
+    else
+        hipLaunchKernelGGL((gn2v::grad_join_kernel<__bf16>), dim3((unsigned)joins), dim3(1024), 0, s, a);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_table_write(const gn2v_table8 *table, const void *d_values, uint32_t dtype, int64_t ldv,
+                     const void *d_ids, uint32_t id_bytes, uint64_t n, int32_t *d_owner, void *stream) {
+    if (check_table(table) || check_ids(d_ids, id_bytes)) return 1;
+    if (dtype != GN2V_F32 && dtype != GN2V_BF16) return fail("unknown dtype");
+    if (n > 0x7FFFFFFFull) return fail("at most 2^31 - 1 entries");
+    if (!d_ids && n > table->rows) return fail("more rows than the table has");
+    if (ldv < (int64_t)table->d) return fail("the row stride must hold a row");
+    if (n == 0 || table->rows == 0) return 0;
+    const bool many = d_ids && n > GN2V_TABLE_FEW_ENTRIES;
+    if (!d_values || (many && !d_owner)) return fail("NULL pointer");
+    DeviceGuard guard(DeviceGuard::of_pointer(table->d_codes));
+    const gn2v::TableView v = table_view(table);
+    hipStream_t s = (hipStream_t)stream;
+    if (many) {
+        const unsigned blocks = (unsigned)std::min<uint64_t>((n + 255) / 256, 256 * 16);
+        for (int clear = 1; clear >= 0; --clear)
+            hipLaunchKernelGGL(gn2v::table_owner_kernel, dim3(blocks), dim3(256), 0, s, d_ids, (int)id_bytes,
+                               n, v.rows, (int *)d_owner, clear);
+    }
+    if (dtype == GN2V_F32)
+        launch_write<float>(table, v, d_values, ldv, d_ids, id_bytes, n, many ? d_owner : nullptr, s);
+    else
+        launch_write<__bf16>(table, v, d_values, ldv, d_ids, id_bytes, n, many ? d_owner : nullptr, s);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_table_read(const gn2v_table8 *table, const void *d_ids, uint32_t id_bytes, uint64_t n,
+                    void *d_out, uint32_t dtype, int64_t ldo, void *stream) {
+    if (check_table(table) || check_ids(d_ids, id_bytes)) return 1;
+    if (dtype != GN2V_F32 && dtype != GN2V_BF16) return fail("unknown dtype");
+    if (ldo < (int64_t)table->d) return fail("the row stride must hold a row");
+    if (n == 0) return 0;
+    if (!d_out) return fail("NULL pointer");
+    DeviceGuard guard(DeviceGuard::of_pointer(d_out));
+    const gn2v::TableView v = table_view(table);
+    if (dtype == GN2V_F32)
+        launch_read<float>(table, v, d_ids, id_bytes, n, d_out, ldo, (hipStream_t)stream);
+    else
+        launch_read<__bf16>(table, v, d_ids, id_bytes, n, d_out, ldo, (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_table_edge_embedding(const gn2v_table8 *src, const gn2v_table8 *dst, const void *d_src_ids,
+                              const void *d_dst_ids, uint32_t id_bytes, uint64_t n_edges,
+                              uint32_t method, float *d_out, int64_t ldo, void *stream) {
+    if (check_table(src) || check_table(dst)) return 1;
+    if (id_bytes != 4 && id_bytes != 8) return fail("id_bytes must be 4 or 8");
+    if (src->d != dst->d || src->code != dst->code) return fail("both tables need the same width and codes");
+    if (method >= gn2v::kEdgeMethodCount) return fail("unknown edge embedding method");
+    const int64_t need = method == gn2v::kConcatenate ? 2 * (int64_t)src->d
+                         : (method == gn2v::kL2Distance || method == gn2v::kCosineSimilarity) ? 1
+                                                                                             : src->d;
+    if (ldo < need) return fail("out row stride is too small for this method");
+    if (n_edges == 0) return 0;
+    if (!d_src_ids || !d_dst_ids || !d_out) return fail("NULL pointer");
+    DeviceGuard guard(DeviceGuard::of_pointer(d_out));
+    const gn2v::TableView a = table_view(src), b = table_view(dst);
+    hipStream_t s = (hipStream_t)stream;
+    switch (method) {
+#define GN2V_EDGES(M)                                                                             \
+    case gn2v::M:                                                                                 \
+        launch_edges<gn2v::M>(src->code, a, b, d_src_ids, d_dst_ids, id_bytes, n_edges, d_out, ldo, s); \
+        break
+        GN2V_EDGES(kHadamard);
+        GN2V_EDGES(kSum);
+        GN2V_EDGES(kAverage);
+        GN2V_EDGES(kL1);
+        GN2V_EDGES(kAbsoluteL1);
+        GN2V_EDGES(kSquaredL2);
+        GN2V_EDGES(kL2);
+        GN2V_EDGES(kConcatenate);
+        GN2V_EDGES(kMin);
+        GN2V_EDGES(kMax);
+        GN2V_EDGES(kL2Distance);
+        GN2V_EDGES(kCosineSimilarity);
+#undef GN2V_EDGES
+    }
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+}  // extern "C"

@@ -5,7 +5,9 @@ from .edge_transformer import METHODS, EdgeTransformer, edge_embedding
 from .graph_transformer import GraphTransformer
 from .node_label_prediction_transformer import NodeLabelPredictionTransformer
 from .node_transformer import NodeTransformer
+from .quantized_table import QuantizedTable
+from .projections import TypePlan, adapted_projection, typed_projection
 
 __all__ = ["EdgeTransformer", "NodeTransformer", "GraphTransformer", "EdgePredictionTransformer",
            "EdgeLabelPredictionTransformer", "NodeLabelPredictionTransformer", "edge_embedding",
-           "METHODS"]
+           "METHODS", "QuantizedTable", "TypePlan", "typed_projection", "adapted_projection"]

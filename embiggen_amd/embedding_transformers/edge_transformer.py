@@ -14,6 +14,7 @@ import pandas as pd
 
 from .. import _lib
 from .node_transformer import NodeTransformer
+from .quantized_table import QuantizedTable, quantized_edge_embedding
 
 METHODS = {
     "Hadamard": 0, "Sum": 1, "Average": 2, "L1": 3, "AbsoluteL1": 4, "SquaredL2": 5, "L2": 6,
@@ -33,7 +34,9 @@ def edge_embedding(table, sources, destinations, method: str = "Hadamard",
                    destination_table=None, embedding_size: Optional[int] = None):
     """out[e] = method(table[sources[e]], destination_table[destinations[e]]) as a float32 CUDA
     tensor.  ``table`` is [N, ld] float32 on the device (``embedding_size`` = number of real
-    columns when the rows are padded); ids are int32 / int64 tensors on the same device."""
+    columns when the rows are padded); ids are int32 / int64 tensors on the same device.  Both tables
+    may be ``QuantizedTable`` instead: their 8-bit rows are read directly (an id outside the table
+    then stands for a row of zeros)."""
     import torch
 
     if method not in METHODS:
@@ -41,6 +44,14 @@ def edge_embedding(table, sources, destinations, method: str = "Hadamard",
             f"The provided edge embedding method `{method}` is not supported. "
             f"The supported methods are {list(METHODS)}."
         )
+    if isinstance(table, QuantizedTable) or isinstance(destination_table, QuantizedTable):
+        if not isinstance(table, QuantizedTable):
+            raise ValueError("Source and destination tables should both be in 8 bits, or neither.")
+        if embedding_size is not None and embedding_size != table.embedding_size:
+            raise ValueError("A table in 8 bits has its own embedding size.")
+        return quantized_edge_embedding(table, sources, destinations, METHODS[method],
+                                        _output_width(method, table.embedding_size),
+                                        destination_table)
     dst_table = table if destination_table is None else destination_table
     if table.dtype != torch.float32 or dst_table.dtype != torch.float32:
         raise ValueError("Embedding tables must be float32.")
@@ -84,8 +95,8 @@ class EdgeTransformer:
 
     The operators run in the fused gather + operator kernel on the node feature table kept in HBM
     (float32); only ids go to the device and only the result comes back.  Device consumers can
-    skip the host altogether: ``fit`` on float32 CUDA tensor(s) and ``transform`` on id tensors
-    returns a CUDA tensor.
+    skip the host altogether: ``fit`` on float32 CUDA tensor(s), or on one ``QuantizedTable``, and
+    ``transform`` on id tensors returns a CUDA tensor.
 
     Deliberate difference: the reference's ``fit`` raises ``ValueError`` for *every* DataFrame
     edge type feature (``if pd.isna(df).any()`` at edge_transformer.py:472 is the truth value of
@@ -113,6 +124,11 @@ class EdgeTransformer:
     # ------------------------------------------------------------------ fit
     def fit(self, node_feature, node_type_feature=None, edge_type_features=None):
         tensors = node_feature if isinstance(node_feature, (list, tuple)) else [node_feature]
+        if any(isinstance(t, QuantizedTable) for t in tensors):
+            if len(tensors) > 1 or node_type_feature is not None or edge_type_features is not None:
+                raise ValueError("A table in 8 bits can only be fitted alone.")
+            self._table = tensors[0]
+            return self
         if len(tensors) and all(_is_tensor(t) for t in tensors):
             # device mode: float32 CUDA tensor(s), hstacked like node_transformer.py:110-116
             import torch

@@ -6,7 +6,8 @@
  * through them and because the parity tests compare every step with the oracle's restatement
  * (oracle/gn2v_oracle.c, "block-partitioned SkipGram") one at a time.  Same conventions as
  * gn2v.h: int status (0 = OK, message in gn2v_last_error), plain pointers and sizes, the
- * caller's stream as void*. */
+ * caller's stream as void*.  At the end: the operators on rows of embedding tables (typed and adapted
+ * products, tables in 8 bits) behind the Python functions of the same names. */
 #ifndef GN2V_INTERNAL_H
 #define GN2V_INTERNAL_H
 
@@ -330,6 +331,117 @@ int gn2v_block_round(gn2v_graph *g, const gn2v_train_params *tp, const gn2v_bloc
  * which calibrates the rocprofv3 FETCH_SIZE / WRITE_SIZE counters (profiles/README.md). */
 int gn2v_touch_rows(float *d_table, uint32_t ld, const uint32_t *d_ids, uint64_t n, uint32_t flags,
                     void *stream);
+
+/* ---- Operators on rows of embedding tables (Python: embiggen_amd.typed_projection,
+ * adapted_projection, QuantizedTable, edge_embedding).  Element types: */
+#define GN2V_F32 0u
+#define GN2V_BF16 1u
+
+/* Rows in the order of their types: a stable counting sort of the type ids (equal types keep the
+ * rows' order).  d_types: int32 or int64 ids (type_bytes 4 / 8); an id outside [0, n_types) -- -1,
+ * the 0xFFFFFFFF of gn2v_graph_set_types read as int32 -- is an unknown type, and its rows come
+ * last.  d_plan int32[plan_words]: order[rows], row_types[rows], offsets[n_types + 2], then the
+ * tiles of the product kernels.  d_temp int32[temp_words] is free again once the launch is over.
+ * rows <= 2^31 - 2^20, 1 <= n_types <= GN2V_MAX_TYPES. */
+#define GN2V_MAX_TYPES 32768u
+#define GN2V_MAX_RANK 64u
+int gn2v_type_plan_words(uint64_t rows, uint32_t n_types, uint64_t *plan_words, uint64_t *temp_words);
+int gn2v_type_plan(const void *d_types, uint32_t type_bytes, uint64_t rows, uint32_t n_types,
+                   int32_t *d_plan, int32_t *d_temp, void *stream);
+
+/* Weights of every type: element (k, n) of type t at t * type_stride + k * inner + n * outer
+ * elements; inner or outer is 1. */
+typedef struct {
+    const void *d_data;
+    int64_t type_stride, inner, outer;
+} gn2v_weights;
+
+typedef struct {
+    uint32_t dtype;       /* GN2V_F32 / GN2V_BF16: x, weights, bias, y                          */
+    uint32_t n_types;
+    uint64_t rows;
+    uint32_t inputs;      /* K                                                                  */
+    uint32_t outputs;     /* N                                                                  */
+    const void *d_x;      /* [rows][ldx], the first K columns                                   */
+    int64_t ldx;
+    gn2v_weights weight;  /* K x N                                                              */
+    const void *d_bias;   /* [type][bias_stride], N columns, or NULL                            */
+    int64_t bias_stride;
+    void *d_y;            /* [rows][ldy]                                                        */
+    int64_t ldy;
+    const int32_t *d_plan;
+    const void *d_types;  /* gn2v_few_rows_product without a plan: the rows' type ids           */
+    uint32_t type_bytes;
+    uint32_t rank;        /* adapted form: <= GN2V_MAX_RANK; 0 = typed form                     */
+    float scale;
+    uint32_t low_rank_rows; /* gn2v_typed_product: y is float32 rows at their POSITIONS in the plan's
+                               order (rows of unknown types are left as they were)              */
+    gn2v_weights down;    /* gn2v_few_rows_product, adapted form: K x rank                      */
+    gn2v_weights up;      /* adapted form: rank x N                                             */
+    const float *d_low;   /* gn2v_adapted_product: [rows][rank] as gn2v_typed_product left them */
+} gn2v_product_io;
+
+/* y[r] = scale * x[r] W[type of r] + bias[type of r]; rows of unknown types are zeros. */
+int gn2v_typed_product(const gn2v_product_io *io, void *stream);
+/* y[r] = x[r] W + bias + low[position of r] up[type of r]; rows of unknown types: the shared part.
+ * low = scale * x[r] down[type of r]: gn2v_typed_product with low_rank_rows. */
+int gn2v_adapted_product(const gn2v_product_io *io, void *stream);
+/* Either form for a few rows (rank 0 / > 0), in one launch and without a plan: every row reads the
+ * whole weights of its type.  inputs <= GN2V_FEW_ROWS_DEPTH, rows <= 65535, weights with outer = 1. */
+#define GN2V_FEW_ROWS_DEPTH 4096u
+int gn2v_few_rows_product(const gn2v_product_io *io, void *stream);
+
+/* Gradients of the weights: dw[t] = sum over the rows r of type t of x[r]^T dy[r], db[t] = sum of
+ * dy[r].  x_low / y_low: that operand is float32 rows at their positions in the plan's order
+ * (else rows of `dtype` at their ids).  shared: one weight for all rows, known type or not.
+ * inputs = 0: db alone.  d_temp: gn2v_typed_gradient_temp bytes.  Sums have a fixed order: the same
+ * bits in every run. */
+typedef struct {
+    uint32_t dtype, n_types;
+    uint64_t rows;
+    uint32_t inputs, outputs;
+    const void *d_x, *d_dy;
+    int64_t ldx, ldy;
+    uint32_t x_low, y_low, shared, reserved;
+    const int32_t *d_plan;
+    void *d_dw; /* [type][inputs][outputs] */
+    void *d_db; /* [type][outputs] or NULL */
+    void *d_temp;
+    uint64_t temp_bytes;
+} gn2v_gradient_io;
+int gn2v_typed_gradient_temp(const gn2v_gradient_io *io, uint64_t *temp_bytes);
+int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream);
+
+/* Embedding tables in 8 bits: codes u8[rows][stride] and a float32 scale per row and group of
+ * `group` (16, 32, 64 or 128) consecutive columns, scales f32[rows][ceil(d / group)]. */
+#define GN2V_INT8 0u
+#define GN2V_E4M3 1u
+typedef struct {
+    void *d_codes;
+    float *d_scales;
+    uint64_t rows;
+    uint32_t d;
+    uint32_t stride; /* bytes between rows: a multiple of 16, >= d; d_codes 16-byte aligned */
+    uint32_t group;
+    uint32_t code;   /* GN2V_INT8 / GN2V_E4M3 */
+} gn2v_table8;
+
+/* Quantises values[i] (GN2V_F32 / GN2V_BF16, row stride ldv) into row ids[i] (int32 / int64 by
+ * id_bytes; NULL: row i) -- scale = max(max |x| / 127 or 448, 2^-90), codes rounded to the nearest,
+ * ties to even; a group with an infinity or a NaN reads back as NaN.  Entries whose id lies outside
+ * the table are left out; of several entries of one row the last is kept.  d_owner int32[rows]:
+ * scratch, needed with ids and n > GN2V_TABLE_FEW_ENTRIES.  n < 2^31. */
+#define GN2V_TABLE_FEW_ENTRIES 1024u
+int gn2v_table_write(const gn2v_table8 *table, const void *d_values, uint32_t dtype, int64_t ldv,
+                     const void *d_ids, uint32_t id_bytes, uint64_t n, int32_t *d_owner, void *stream);
+/* out[i] = row ids[i] (NULL: row i), zeros where the id lies outside the table. */
+int gn2v_table_read(const gn2v_table8 *table, const void *d_ids, uint32_t id_bytes, uint64_t n,
+                    void *d_out, uint32_t dtype, int64_t ldo, void *stream);
+/* gn2v_edge_embedding on two tables in 8 bits of the same width and code (float32 results); an id
+ * outside its table stands for a row of zeros. */
+int gn2v_table_edge_embedding(const gn2v_table8 *src, const gn2v_table8 *dst, const void *d_src_ids,
+                              const void *d_dst_ids, uint32_t id_bytes, uint64_t n_edges,
+                              uint32_t method, float *d_out, int64_t ldo, void *stream);
 
 #ifdef __cplusplus
 }
