@@ -16,23 +16,25 @@ namespace {
 
 constexpr uint64_t kMaxRows = (1ull << 31) - (1ull << 20);  // positions are int32
 
-// the plan's words and the stripes its rows are counted in
+// the plan's words, and the stripes its rows are counted in
 struct PlanSizes {
-    uint64_t tile_bound, words, temp;
+    uint64_t words, temp;
     uint32_t stripes, stripe;
 };
 
 PlanSizes plan_sizes(uint64_t rows, uint32_t types) {
     PlanSizes s;
-    s.tile_bound = std::min<uint64_t>(rows, (rows + 63) / 64 + std::min<uint64_t>(types + 1ull, rows));
-    s.words = (2 * rows + types + 2 + 1) / 2 * 2 + 2 * s.tile_bound;
-    // one wave each: 512 rows at least, and at most 4 M counters in all
-    uint64_t stripes = std::min<uint64_t>((rows + 511) / 512, 4096);
-    stripes = std::max<uint64_t>(1, std::min<uint64_t>(stripes, (1ull << 22) / (types + 1)));
-    s.stripe = (uint32_t)(((rows + stripes - 1) / stripes + 63) / 64 * 64);
-    s.stripes = s.stripe ? (uint32_t)((rows + s.stripe - 1) / s.stripe) : 0;
-    s.temp = rows <= gn2v::kSmallPlan ? 0 : (uint64_t)s.stripes * (types + 1) + types + 1;
+    s.words = 2 * rows + 2 * (types + 2ull);
+    const uint64_t stripe = std::max<uint64_t>(1024, (rows + gn2v::kStripes - 1) / gn2v::kStripes);
+    s.stripe = (uint32_t)((stripe + 255) / 256 * 256);
+    s.stripes = (uint32_t)((rows + s.stripe - 1) / s.stripe);
+    s.temp = rows <= gn2v::kSmallPlan ? 0 : (s.stripes + 1ull) * (types + 1ull);
     return s;
+}
+
+// tiles of at most 64 rows of one type, unknown rows among the types
+uint64_t tile_bound(uint64_t rows, uint64_t groups) {
+    return std::min<uint64_t>(rows, (rows + gn2v::kTileRows - 1) / gn2v::kTileRows + std::min(groups, rows));
 }
 
 gn2v::PlanView plan_view(const int32_t *d_plan, uint64_t rows, uint32_t types) {
@@ -44,8 +46,7 @@ gn2v::PlanView plan_view(const int32_t *d_plan, uint64_t rows, uint32_t types) {
     v.order = p;
     v.row_types = p + rows;
     v.offsets = p + 2 * rows;
-    v.tile_bound = (uint32_t)plan_sizes(rows, types).tile_bound;
-    v.tiles = reinterpret_cast<int2 *>(p + (2 * rows + types + 2 + 1) / 2 * 2);
+    v.tile_first = v.offsets + types + 2;
     return v;
 }
 
@@ -63,6 +64,13 @@ int alignment(const void *base, int64_t stride_elements, uint32_t size) {
     return (int)(bits & (~bits + 1));
 }
 
+// how the chunks of rows of `length` elements are loaded (ChunkMode)
+int mode_of(const void *base, int64_t stride, uint32_t length, uint32_t size, int64_t type_stride = 0) {
+    const int align = std::min(alignment(base, stride, size), alignment(nullptr, type_stride, size));
+    if (align == 16 && length % (16 / size) == 0) return gn2v::kWhole;
+    return size == 4 || (align >= 4 && length % 2 == 0) ? gn2v::kWords : gn2v::kElements;
+}
+
 template <typename I>
 void launch_plan(const I *types, const gn2v::PlanView &v, int32_t *temp, hipStream_t s) {
     if (v.rows <= gn2v::kSmallPlan) {
@@ -70,24 +78,25 @@ void launch_plan(const I *types, const gn2v::PlanView &v, int32_t *temp, hipStre
         return;
     }
     const PlanSizes z = plan_sizes(v.rows, v.types);
-    const size_t lds = (v.types + 1) * sizeof(int);
-    if (lds > 65536) {  // more than 16 383 types: the counters need more than the default limit
+    const uint32_t groups = v.types + 1;
+    // four waves a workgroup while their counters fit 64 KB, one wave with up to 128 KB of them else
+    const unsigned waves = groups <= 4096 ? 4 : 1, threads = 64 * waves;
+    const size_t lds = groups * sizeof(int);
+    if (lds * waves > 65536) {  // more than the default limit
         (void)hipFuncSetAttribute((const void *)gn2v::plan_count_kernel<I>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         (void)hipFuncSetAttribute((const void *)gn2v::plan_place_kernel<I>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)(lds * waves));
     }
-    int *counts = temp, *totals = temp + (uint64_t)z.stripes * (v.types + 1);
-    hipLaunchKernelGGL((gn2v::plan_count_kernel<I>), dim3(z.stripes), dim3(64), lds, s, types, v.rows,
-                       v.types, z.stripe, z.stripes, counts);
-    hipLaunchKernelGGL(gn2v::plan_scan_kernel, dim3(v.types + 1), dim3(256), 0, s, counts, z.stripes,
-                       totals);
-    hipLaunchKernelGGL(gn2v::plan_pieces_kernel, dim3(1), dim3(1024), 0, s, totals, v.offsets,
-                       v.types + 1, (uint32_t)gn2v::kTileRows, v.tile_bound, v.tiles, (int *)nullptr);
+    int *counts = temp, *totals = temp + (uint64_t)z.stripes * groups;
+    hipLaunchKernelGGL((gn2v::plan_count_kernel<I>), dim3(z.stripes), dim3(256), lds, s, types, v.rows,
+                       v.types, z.stripe, counts);
+    hipLaunchKernelGGL(gn2v::plan_scan_kernel, dim3((groups + 3) / 4), dim3(256), 0, s, counts, z.stripes,
+                       groups, totals);
     int bits = 0;
     while (v.types >> bits) ++bits;
-    hipLaunchKernelGGL((gn2v::plan_place_kernel<I>), dim3(z.stripes), dim3(64), lds, s, types, v,
-                       z.stripe, z.stripes, counts, bits);
+    hipLaunchKernelGGL((gn2v::plan_place_kernel<I>), dim3(z.stripes), dim3(threads), lds * waves, s, types,
+                       v, z.stripe, z.stripes, counts, bits, totals);
 }
 
 int check_product(const gn2v_product_io *io) {
@@ -105,10 +114,11 @@ int check_product(const gn2v_product_io *io) {
     return 0;
 }
 
-gn2v::WeightView view_of(const gn2v_weights &w, uint32_t size) {
+// weights of `inputs` x `outputs`
+gn2v::WeightView view_of(const gn2v_weights &w, uint32_t inputs, uint32_t outputs, uint32_t size) {
     gn2v::WeightView v{w.d_data, w.type_stride, w.inner, w.outer, 0};
     const int64_t row = w.outer == 1 ? w.inner : w.outer;
-    v.align = std::min(alignment(w.d_data, row, size), alignment(nullptr, w.type_stride, size));
+    v.mode = mode_of(w.d_data, row, w.outer == 1 ? outputs : inputs, size, w.type_stride);
     return v;
 }
 
@@ -117,15 +127,14 @@ gn2v::ProductArgs product_args(const gn2v_product_io *io) {
     gn2v::ProductArgs a{};
     a.x = io->d_x;
     a.ldx = io->ldx;
-    a.x_align = alignment(io->d_x, io->ldx, size);
-    a.w = view_of(io->weight, size);
+    a.x_mode = mode_of(io->d_x, io->ldx, io->inputs, size);
+    a.w = view_of(io->weight, io->inputs, io->outputs, size);
     a.bias = io->d_bias;
     a.bias_type = io->bias_stride;
     a.y = io->d_y;
     a.ldy = io->ldy;
     a.sorted = io->low_rank_rows != 0;
-    const uint32_t out = a.sorted ? 4 : size;
-    a.y_vec = alignment(io->d_y, io->ldy, out) >= (int)(4 * out);
+    a.y_align = alignment(io->d_y, io->ldy, a.sorted ? 4 : size);
     a.scale = io->scale;
     a.plan = plan_view(io->d_plan, io->rows, io->n_types);
     a.K = (int)io->inputs;
@@ -133,10 +142,13 @@ gn2v::ProductArgs product_args(const gn2v_product_io *io) {
     return a;
 }
 
+uint64_t product_tiles(const gn2v::ProductArgs &a, bool any_type) {
+    return any_type ? (a.plan.rows + 63) / 64 : tile_bound(a.plan.rows, a.plan.types + 1ull);
+}
+
 template <typename T, int BN, bool WT, bool ADAPT>
 void launch_product_kernel(const gn2v::ProductArgs &a, hipStream_t s) {
-    const uint64_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : a.plan.tile_bound;
-    const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8 * ((a.N + BN - 1) / BN));
+    const unsigned blocks = (unsigned)((product_tiles(a, ADAPT) + 7) / 8 * 8 * ((a.N + BN - 1) / BN));
     hipLaunchKernelGGL((gn2v::product_kernel<T, BN, WT, ADAPT>), dim3(blocks), dim3(256), 0, s, a);
 }
 
@@ -150,24 +162,61 @@ void launch_product_bn(const gn2v::ProductArgs &a, hipStream_t s) {
         launch_product_kernel<T, 128, WT, ADAPT>(a, s);
 }
 
-template <bool ADAPT>
-int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, hipStream_t s) {
-    const uint64_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : a.plan.tile_bound;
-    if (((tiles + 7) / 8 * 8) * ((a.N + 31) / 32) > 0x7FFFFFFFull) return fail("too many tiles for one launch");
-    const bool wt = a.w.outer != 1;
-    if (dtype == GN2V_F32)
-        wt ? launch_product_bn<float, true, ADAPT>(a, s) : launch_product_bn<float, false, ADAPT>(a, s);
+template <typename T, int SLABS, int BN, bool WT, bool ADAPT>
+void launch_narrow_kernel(gn2v::ProductArgs a, hipStream_t s) {
+    // as many workgroups as are resident at once: two per CU
+    const unsigned columns = (unsigned)((a.N + BN - 1) / BN);
+    a.ranges = (uint32_t)std::min<uint64_t>(product_tiles(a, false), std::max(512u / columns, 64u));
+    hipLaunchKernelGGL((gn2v::narrow_product_kernel<T, SLABS, BN, WT, ADAPT>),
+                       dim3((a.ranges + 7) / 8 * 8 * columns), dim3(gn2v::kNarrowThreads), 0, s, a);
+}
+
+template <typename T, int SLABS, bool WT, bool ADAPT>
+void launch_narrow_bn(const gn2v::ProductArgs &a, hipStream_t s) {
+    if (a.N <= 64)
+        launch_narrow_kernel<T, SLABS, 64, WT, ADAPT>(a, s);
     else
+        launch_narrow_kernel<T, SLABS, 128, WT, ADAPT>(a, s);
+}
+
+template <typename T, bool WT, bool ADAPT>
+void launch_narrow(const gn2v::ProductArgs &a, hipStream_t s) {
+    constexpr int slab = gn2v::Tile<T>::kSlab;
+    if (a.K <= 2 * slab)
+        launch_narrow_bn<T, 2, WT, ADAPT>(a, s);
+    else if (a.K <= 4 * slab)
+        launch_narrow_bn<T, 4, WT, ADAPT>(a, s);
+    else
+        launch_narrow_bn<T, 8, WT, ADAPT>(a, s);
+}
+
+// rows whose inner elements fit the narrow kernel's LDS tile
+bool is_narrow(uint32_t dtype, uint32_t inputs) { return inputs <= (dtype == GN2V_F32 ? 128u : 256u); }
+
+template <bool ADAPT>
+int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, bool narrow, hipStream_t s) {
+    if ((product_tiles(a, false) + 7) / 8 * 8 * ((a.N + 31) / 32) > 0x7FFFFFFFull)
+        return fail("too many tiles for one launch");
+    const bool wt = a.w.outer != 1;
+    if (narrow) {
+        if (dtype == GN2V_F32)
+            wt ? launch_narrow<float, true, ADAPT>(a, s) : launch_narrow<float, false, ADAPT>(a, s);
+        else
+            wt ? launch_narrow<__bf16, true, ADAPT>(a, s) : launch_narrow<__bf16, false, ADAPT>(a, s);
+    } else if (dtype == GN2V_F32) {
+        wt ? launch_product_bn<float, true, ADAPT>(a, s) : launch_product_bn<float, false, ADAPT>(a, s);
+    } else {
         wt ? launch_product_bn<__bf16, true, ADAPT>(a, s) : launch_product_bn<__bf16, false, ADAPT>(a, s);
+    }
     HIP_TRY(hipGetLastError());
     return 0;
 }
 
-// how the rows of a gradient are cut: about 1024 workgroups over the chunks and blocks of dw, pieces
-// of 128 rows at least, and no more than 256 MB of partial sums beside the one per type
+// How a gradient's tiles are dealt out: to as many workgroups as are resident at once over the blocks
+// of dw, with no more than 256 MB of partial sums.
 struct GradSizes {
-    uint32_t bm, bn, chunk_rows;
-    uint64_t chunks, stride, list_words, bytes;
+    uint32_t bm, bn, ranges;
+    uint64_t stride, bytes;
 };
 
 GradSizes grad_sizes(const gn2v_gradient_io *io) {
@@ -176,17 +225,12 @@ GradSizes grad_sizes(const gn2v_gradient_io *io) {
     g.bn = io->outputs <= 32 ? 32 : io->outputs <= 64 ? 64 : 128;
     const uint64_t blocks = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm) * ((io->outputs + g.bn - 1) / g.bn);
     g.stride = (((uint64_t)io->inputs + 1) * io->outputs + 3) / 4 * 4;
-    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>((1024 + blocks - 1) / blocks, (64ull << 20) / g.stride));
-    uint64_t rows = (io->rows + most - 1) / most;
-    rows = std::max<uint64_t>(128, (rows + 63) / 64 * 64);
-    g.chunk_rows = (uint32_t)rows;
-    g.chunks = (io->rows + rows - 1) / rows;
-    g.list_words = 0;
-    if (!io->shared) {
-        g.chunks += std::min<uint64_t>(io->n_types, io->rows);
-        g.list_words = (2 * g.chunks + io->n_types + 1 + 3) / 4 * 4;
-    }
-    g.bytes = g.list_words * 4 + g.chunks * g.stride * 4;
+    const uint64_t tiles = tile_bound(io->rows, io->shared ? 0 : io->n_types);
+    const uint64_t resident = 256u * gn2v::grad_waves(g.bm / 32, g.bn / 32);
+    uint64_t ranges = std::min<uint64_t>(std::max<uint64_t>(1, resident / blocks), (32ull << 20) / g.stride);
+    ranges = std::max<uint64_t>(1, std::min(ranges, tiles));
+    g.ranges = (uint32_t)ranges;
+    g.bytes = io->rows ? 2 * ranges * g.stride * 4 : 0;
     return g;
 }
 
@@ -279,41 +323,42 @@ int check_ids(const void *ids, uint32_t id_bytes) {
 template <typename T>
 void launch_write(const gn2v_table8 *t, const gn2v::TableView &v, const void *values, int64_t ldv,
                   const void *ids, uint32_t id_bytes, uint64_t n, const int32_t *owner, hipStream_t s) {
-    const int shift = lanes_shift(t->d), align = alignment(values, ldv, sizeof(T));
+    const int shift = lanes_shift(t->d), mode = mode_of(values, ldv, t->d, sizeof(T));
     const unsigned blocks = row_blocks(n, shift);
     if (t->code == GN2V_INT8)
         hipLaunchKernelGGL((gn2v::table_write_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v,
-                           (const T *)values, ldv, align, ids, (int)id_bytes, n, owner, shift);
+                           (const T *)values, ldv, mode, ids, (int)id_bytes, n, owner, shift);
     else
         hipLaunchKernelGGL((gn2v::table_write_kernel<T, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, v,
-                           (const T *)values, ldv, align, ids, (int)id_bytes, n, owner, shift);
+                           (const T *)values, ldv, mode, ids, (int)id_bytes, n, owner, shift);
 }
 
 template <typename T>
 void launch_read(const gn2v_table8 *t, const gn2v::TableView &v, const void *ids, uint32_t id_bytes,
                  uint64_t n, void *out, int64_t ldo, hipStream_t s) {
-    const int shift = lanes_shift(t->d), vec = alignment(out, ldo, sizeof(T)) == 16;
+    const int shift = lanes_shift(t->d), align = alignment(out, ldo, sizeof(T));
     const unsigned blocks = row_blocks(n, shift);
     if (t->code == GN2V_INT8)
         hipLaunchKernelGGL((gn2v::table_read_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v, ids,
-                           (int)id_bytes, n, (T *)out, ldo, vec, shift);
+                           (int)id_bytes, n, (T *)out, ldo, align, shift);
     else
         hipLaunchKernelGGL((gn2v::table_read_kernel<T, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, v, ids,
-                           (int)id_bytes, n, (T *)out, ldo, vec, shift);
+                           (int)id_bytes, n, (T *)out, ldo, align, shift);
 }
 
 template <uint32_t METHOD>
 void launch_edges(uint32_t code, const gn2v::TableView &a, const gn2v::TableView &b, const void *u,
                   const void *w, uint32_t id_bytes, uint64_t n, float *out, int64_t ldo, hipStream_t s) {
     const int shift = lanes_shift(a.d);
-    const int vec = alignment(out, ldo, 4) == 16 && (METHOD != gn2v::kConcatenate || (a.d & 3) == 0);
+    // Concatenate's second half starts behind the first
+    const int align = std::min(alignment(out, ldo, 4), METHOD == gn2v::kConcatenate ? alignment(out, a.d, 4) : 16);
     const unsigned blocks = row_blocks(n, shift);
     if (code == GN2V_INT8)
         hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, a,
-                           b, u, w, (int)id_bytes, n, out, ldo, vec, shift);
+                           b, u, w, (int)id_bytes, n, out, ldo, align, shift);
     else
         hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, a,
-                           b, u, w, (int)id_bytes, n, out, ldo, vec, shift);
+                           b, u, w, (int)id_bytes, n, out, ldo, align, shift);
 }
 
 }  // namespace
@@ -350,7 +395,8 @@ int gn2v_typed_product(const gn2v_product_io *io, void *stream) {
     if (io->rows == 0) return 0;
     if (!io->d_plan) return fail("NULL plan");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
-    return launch_product<false>(io->dtype, product_args(io), (hipStream_t)stream);
+    return launch_product<false>(io->dtype, product_args(io), !io->low_rank_rows && is_narrow(io->dtype, io->inputs),
+                                 (hipStream_t)stream);
 }
 
 int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
@@ -358,17 +404,35 @@ int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
     if (io->rank == 0) return fail("need a rank of at least 1");
     if (io->low_rank_rows) return fail("low_rank_rows belongs to gn2v_typed_product");
     if (io->rows == 0) return 0;
-    if (!io->d_plan || !io->d_low || !io->up.d_data) return fail("NULL pointer");
-    if ((io->weight.outer == 1) != (io->up.outer == 1) && io->rank > 1)
+    if (!io->d_plan || !io->down.d_data || !io->up.d_data) return fail("NULL pointer");
+    const bool narrow = io->rank <= gn2v::kFusedRank && is_narrow(io->dtype, io->inputs);
+    if (!narrow && !io->d_low) return fail("NULL low-rank rows");
+    if (!narrow && (io->weight.outer == 1) != (io->up.outer == 1) && io->rank > 1)
         return fail("weight and up must be laid out alike");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
+    const uint32_t size = size_of(io->dtype);
     gn2v::ProductArgs a = product_args(io);
-    a.scale = 1.f;  // the low-rank rows hold it
     a.bias_type = 0;
-    a.low = io->d_low;
     a.rank = (int)io->rank;
-    a.up = view_of(io->up, size_of(io->dtype));
-    return launch_product<true>(io->dtype, a, (hipStream_t)stream);
+    a.down = view_of(io->down, io->inputs, io->rank, size);
+    a.up = view_of(io->up, io->rank, io->outputs, size);
+    a.low_out = io->d_low;
+    hipStream_t s = (hipStream_t)stream;
+    if (!narrow) {
+        // the low-rank rows first, by the typed product
+        gn2v::ProductArgs low = a;
+        low.w = a.down;
+        low.bias = nullptr;
+        low.y = io->d_low;
+        low.ldy = (int64_t)io->rank;
+        low.y_align = alignment(io->d_low, (int64_t)io->rank, 4);
+        low.sorted = 1;
+        low.N = (int)io->rank;
+        if (launch_product<false>(io->dtype, low, false, s)) return 1;
+        a.low = io->d_low;
+        a.scale = 1.f;  // the low-rank rows hold it
+    }
+    return launch_product<true>(io->dtype, a, narrow, s);
 }
 
 int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
@@ -387,7 +451,7 @@ int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
     gn2v::FewArgs a{};
     a.x = io->d_x;
     a.ldx = io->ldx;
-    a.w = view_of(io->weight, size);
+    a.w = view_of(io->weight, io->inputs, io->outputs, size);
     a.bias = io->d_bias;
     a.bias_type = io->bias_stride;
     a.y = io->d_y;
@@ -402,8 +466,8 @@ int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
     const dim3 grid((io->outputs + 63) / 64, (unsigned)io->rows);
     hipStream_t s = (hipStream_t)stream;
     if (io->rank) {
-        a.down = view_of(io->down, size);
-        a.up = view_of(io->up, size);
+        a.down = view_of(io->down, io->inputs, io->rank, size);
+        a.up = view_of(io->up, io->rank, io->outputs, size);
         if (io->dtype == GN2V_F32)
             hipLaunchKernelGGL((gn2v::few_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
         else
@@ -434,7 +498,7 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
     const GradSizes g = grad_sizes(io);
     if (io->temp_bytes < g.bytes || (g.bytes && !io->d_temp)) return fail("d_temp is too small");
     const uint64_t kb = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm), nb = (io->outputs + g.bn - 1) / g.bn;
-    const uint64_t blocks = (g.chunks + 7) / 8 * 8 * kb * nb;
+    const uint64_t blocks = (g.ranges + 7ull) / 8 * 8 * kb * nb;
     const uint32_t types = io->shared ? 1 : io->n_types;
     const uint64_t joins = types * ((g.stride + 255) / 256);
     if (blocks > 0x7FFFFFFFull || joins > 0x7FFFFFFFull) return fail("too many blocks for one launch");
@@ -446,29 +510,18 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
     a.dy = io->d_dy;
     a.ldx = io->ldx;
     a.ldy = io->ldy;
-    a.x_align = alignment(io->d_x, io->ldx, io->x_low ? 4 : size);
-    a.y_align = alignment(io->d_dy, io->ldy, io->y_low ? 4 : size);
-    const gn2v::PlanView v = plan_view(io->d_plan, io->rows, io->n_types);
-    a.rows = (uint32_t)io->rows;
+    a.x_mode = mode_of(io->d_x, io->ldx, io->inputs, io->x_low ? 4 : size);
+    a.y_mode = mode_of(io->d_dy, io->ldy, io->outputs, io->y_low ? 4 : size);
+    a.plan = plan_view(io->d_plan, io->rows, io->n_types);
+    a.shared = io->shared != 0;
     a.types = types;
-    a.chunk_rows = g.chunk_rows;
-    a.chunk_bound = (uint32_t)g.chunks;
+    a.ranges = g.ranges;
     a.K = (int)io->inputs;
     a.N = (int)io->outputs;
     a.stride = (int64_t)g.stride;
+    a.partial = (float *)io->d_temp;
     a.dw = io->d_dw;
     a.db = io->d_db;
-    a.partial = (float *)((char *)io->d_temp + g.list_words * 4);
-    if (!io->shared && io->rows) {
-        int2 *chunks = (int2 *)io->d_temp;
-        int *first = (int *)(chunks + g.chunks);
-        hipLaunchKernelGGL(gn2v::plan_pieces_kernel, dim3(1), dim3(1024), 0, s, (const int *)nullptr,
-                           v.offsets, io->n_types, g.chunk_rows, (uint32_t)g.chunks, chunks, first);
-        a.order = v.order;
-        a.offsets = v.offsets;
-        a.chunks = chunks;
-        a.first = first;
-    }
     if (io->rows) {
         if (io->dtype == GN2V_F32)
             launch_grad<float>(io, g, a, (unsigned)blocks, s);
@@ -476,10 +529,12 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
             launch_grad<__bf16>(io, g, a, (unsigned)blocks, s);
         HIP_TRY(hipGetLastError());
     }
+    // few types lie in many ranges each: sixteen waves share them, four where there are many types
+    const unsigned threads = types >= 64 ? 256 : 1024;
     if (io->dtype == GN2V_F32)
-        hipLaunchKernelGGL((gn2v::grad_join_kernel<float>), dim3((unsigned)joins), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL((gn2v::grad_join_kernel<float>), dim3((unsigned)joins), dim3(threads), 0, s, a);
     else
-        hipLaunchKernelGGL((gn2v::grad_join_kernel<__bf16>), dim3((unsigned)joins), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL((gn2v::grad_join_kernel<__bf16>), dim3((unsigned)joins), dim3(threads), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
 }

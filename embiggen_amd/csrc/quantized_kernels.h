@@ -88,18 +88,18 @@ __device__ __forceinline__ int64_t table_row(const void *ids, int id_bytes, uint
     return r >= 0 && (uint64_t)r < rows ? r : -1;
 }
 
-// eight consecutive elements of a row as float32, zeros from element `valid` on
+// elements c .. c + 7 of a row of d as float32, zeros behind its end
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, int valid, int align, float *v) {
+__device__ __forceinline__ void load8(const T *row, int c, int d, int mode, float *v) {
     if constexpr (sizeof(T) == 4) {
-        const u32x4 a = load_chunk(p, valid, align), b = load_chunk(p + 4, valid - 4, align);
+        const u32x4 a = load_chunk(row, c, d, mode), b = load_chunk(row, c + 4, d, mode);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[i] = __uint_as_float(a[i]);
             v[4 + i] = __uint_as_float(b[i]);
         }
     } else {
-        const u32x4 a = load_chunk(p, valid, align);
+        const u32x4 a = load_chunk(row, c, d, mode);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             v[i] = __uint_as_float(i & 1 ? a[i / 2] & 0xFFFF0000u : a[i / 2] << 16);
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void table_owner_kernel(const void *ids, int i
 // `lanes` lanes per row (a power of two up to 64), eight columns per lane and step.
 template <typename T, uint32_t CODE>
 __global__ __launch_bounds__(256) void table_write_kernel(TableView t, const T *__restrict__ values,
-                                                          int64_t ldv, int align, const void *ids,
+                                                          int64_t ldv, int mode, const void *ids,
                                                           int id_bytes, uint64_t n, const int *owner,
                                                           int lanes_shift) {
     const int lane = threadIdx.x & ((1 << lanes_shift) - 1);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void table_write_kernel(TableView t, const T *
         for (uint32_t c0 = 0; c0 < t.stride; c0 += 8u << lanes_shift) {
             const uint32_t c = c0 + 8 * lane;
             float x[8] = {};
-            if (r >= 0 && c < t.d) load8(values + (int64_t)i * ldv + c, (int)(t.d - c), align, x);
+            if (r >= 0 && c < t.d) load8(values + (int64_t)i * ldv, (int)c, (int)t.d, mode, x);
             uint32_t top = 0;  // as bits: NaN lies above infinity above the numbers
 #pragma unroll
             for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
@@ -183,32 +183,10 @@ __device__ __forceinline__ void table_chunk(const TableView &t, int64_t r, uint3
     }
 }
 
-// eight consecutive output elements, `valid` of them inside the row
-__device__ __forceinline__ void store8(float *p, const float *v, int valid, bool vec) {
-    if (vec && valid >= 8) {
-        reinterpret_cast<f32x4 *>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-        reinterpret_cast<f32x4 *>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
-        return;
-    }
-    store4(p, f32x4{v[0], v[1], v[2], v[3]}, valid, vec);
-    store4(p + 4, f32x4{v[4], v[5], v[6], v[7]}, valid - 4, vec);
-}
-__device__ __forceinline__ void store8(__bf16 *p, const float *v, int valid, bool vec) {
-    if (vec && valid >= 8) {
-        bf16x8 h;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = to_bf16(v[i]);
-        *reinterpret_cast<bf16x8 *>(p) = h;
-        return;
-    }
-    store4(p, f32x4{v[0], v[1], v[2], v[3]}, valid, false);
-    store4(p + 4, f32x4{v[4], v[5], v[6], v[7]}, valid - 4, false);
-}
-
 template <typename T, uint32_t CODE>
 __global__ __launch_bounds__(256) void table_read_kernel(TableView t, const void *ids, int id_bytes,
                                                          uint64_t n, T *__restrict__ out, int64_t ldo,
-                                                         int vec, int lanes_shift) {
+                                                         int align, int lanes_shift) {
     const int lane = threadIdx.x & ((1 << lanes_shift) - 1);
     const uint64_t entries = ((uint64_t)gridDim.x * 256) >> lanes_shift;
     for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_shift; i < n; i += entries) {
@@ -216,7 +194,7 @@ __global__ __launch_bounds__(256) void table_read_kernel(TableView t, const void
         for (uint32_t c = 8 * lane; c < t.d; c += 8u << lanes_shift) {
             float v[8];
             table_chunk<CODE>(t, r, c, v);
-            store8(out + (int64_t)i * ldo + c, v, (int)(t.d - c), vec);
+            store8(out + (int64_t)i * ldo + c, v, (int)(t.d - c), align);
         }
     }
 }
@@ -226,7 +204,7 @@ template <uint32_t METHOD, uint32_t CODE>
 __global__ __launch_bounds__(256) void table_edges_kernel(TableView src, TableView dst,
                                                           const void *src_ids, const void *dst_ids,
                                                           int id_bytes, uint64_t n,
-                                                          float *__restrict__ out, int64_t ldo, int vec,
+                                                          float *__restrict__ out, int64_t ldo, int align,
                                                           int lanes_shift) {
     constexpr bool kReduce = METHOD == kL2Distance || METHOD == kCosineSimilarity;
     const int lane = threadIdx.x & ((1 << lanes_shift) - 1);
@@ -277,8 +255,8 @@ __global__ __launch_bounds__(256) void table_edges_kernel(TableView src, TableVi
             }
             if constexpr (!kReduce) {
                 if (live) {
-                    store8(o + c, v, (int)(src.d - c), vec);
-                    if constexpr (METHOD == kConcatenate) store8(o + src.d + c, b, (int)(src.d - c), vec);
+                    store8(o + c, v, (int)(src.d - c), align);
+                    if constexpr (METHOD == kConcatenate) store8(o + src.d + c, b, (int)(src.d - c), align);
                 }
             }
         }

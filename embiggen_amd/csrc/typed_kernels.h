@@ -25,12 +25,11 @@ constexpr int kSmallPlan = 1024;  // rows one workgroup sorts in LDS
 // ------------------------------------------------------------------------------------ the plan
 // int32 words: order[rows] (row id at every position), row_types[rows] (type at every position;
 // n_types = unknown: any id outside [0, n_types); those rows come last), offsets[n_types + 2]
-// (first position of every type, of the unknown rows, rows), tiles[2 * tile_bound] (type, first
-// position) with type -1 behind the last one.
+// (first position of every type, of the unknown rows, rows), tile_first[n_types + 2] (the same in
+// tiles: a type of c rows has ceil(c / 64) of them).
 struct PlanView {
-    int *order, *row_types, *offsets;
-    int2 *tiles;
-    uint32_t rows, types, tile_bound;
+    int *order, *row_types, *offsets, *tile_first;
+    uint32_t rows, types;
 };
 
 template <typename I>
@@ -39,14 +38,15 @@ __device__ __forceinline__ int type_at(const I *types, uint32_t row, uint32_t n_
     return t >= 0 && (uint64_t)t < (uint64_t)n_types ? (int)t : (int)n_types;
 }
 
-// Up to 1 024 rows: one workgroup sorts (type << 10 | row) in LDS -- a launch instead of four.
+// Up to 1 024 rows: one workgroup sorts (type << 10 | row) in LDS -- one launch.
 template <typename I>
 __global__ __launch_bounds__(kSmallPlan) void plan_small_kernel(const I *__restrict__ types, PlanView p) {
     __shared__ uint32_t key[kSmallPlan];
+    __shared__ int tiles[kSmallPlan + 1];  // tile starts before every position
     __shared__ int wave_sum[kSmallPlan / 64];
     const uint32_t i = threadIdx.x;
     key[i] = i < p.rows ? (uint32_t)type_at(types, i, p.types) << 10 | i : 0xFFFFFFFFu;
-    uint32_t n = 64;  // every wave takes part; the sort covers the smallest power of two
+    uint32_t n = 64;  // the sort covers the smallest power of two
     while (n < p.rows) n <<= 1;
     for (uint32_t size = 2; size <= n; size <<= 1)
         for (uint32_t step = size >> 1; step; step >>= 1) {
@@ -73,168 +73,214 @@ __global__ __launch_bounds__(kSmallPlan) void plan_small_kernel(const I *__restr
         return lo;
     };
     bool starts = false;
-    uint32_t type = 0;
     if (i < p.rows) {
-        type = key[i] >> 10;
+        const uint32_t type = key[i] >> 10;
         p.order[i] = (int)(key[i] & 1023u);
         p.row_types[i] = (int)type;
         starts = (i - first_of(type)) % kTileRows == 0;
     }
-    for (uint32_t t = i; t < p.types + 2; t += kSmallPlan)
-        p.offsets[t] = t <= p.types ? (int)first_of(t) : (int)p.rows;
     const unsigned long long ballot = __ballot(starts);
     if ((i & 63) == 0) wave_sum[i >> 6] = __popcll(ballot);
     __syncthreads();
-    int at = 0, total = 0;
-    for (uint32_t w = 0; w < kSmallPlan / 64; ++w) {
-        if (w < i >> 6) at += wave_sum[w];
-        total += wave_sum[w];
+    int at = __popcll(ballot & ((1ull << (i & 63)) - 1));
+    for (uint32_t w = 0; w < i >> 6; ++w) at += wave_sum[w];
+    tiles[i] = at;
+    if (i == kSmallPlan - 1) tiles[kSmallPlan] = at + starts;
+    __syncthreads();
+    for (uint32_t t = i; t < p.types + 2; t += kSmallPlan) {
+        const uint32_t first = t <= p.types ? first_of(t) : p.rows;
+        p.offsets[t] = (int)first;
+        p.tile_first[t] = tiles[first];
     }
-    at += __popcll(ballot & ((1ull << (i & 63)) - 1));
-    if (starts) p.tiles[at] = make_int2((int)type, (int)i);
-    for (uint32_t t = i; t < p.tile_bound; t += kSmallPlan)
-        if (t >= (uint32_t)total) p.tiles[t] = make_int2(-1, 0);
 }
 
-// More rows: one wave per stripe of rows counts its types in LDS, the counts are scanned per type and
-// over the types, and the same wave places its rows.  Equal types keep their rows' order (a wave
-// ranks its 64 rows by ballots over the bits of their types), so sums over a type's rows have the
-// same order in every run.
+// More rows: a workgroup per stripe of rows counts its types in LDS; the counts of the stripes before
+// it and of the smaller types say where its rows go.  Equal types keep their rows' order (a wave
+// takes a part of the stripe in order and ranks 64 rows at a time by ballots over the bits of their
+// types), so sums over a type's rows have the same order in every run.
 template <typename I>
-__global__ __launch_bounds__(64) void plan_count_kernel(const I *__restrict__ types, uint32_t rows,
-                                                        uint32_t n_types, uint32_t stripe,
-                                                        uint32_t stripes, int *__restrict__ counts) {
+__global__ __launch_bounds__(256) void plan_count_kernel(const I *__restrict__ types, uint32_t rows,
+                                                         uint32_t n_types, uint32_t stripe,
+                                                         int *__restrict__ counts) {
     extern __shared__ int count[];
-    for (uint32_t t = threadIdx.x; t <= n_types; t += 64) count[t] = 0;
+    for (uint32_t t = threadIdx.x; t <= n_types; t += blockDim.x) count[t] = 0;
     __syncthreads();
     const uint64_t first = (uint64_t)blockIdx.x * stripe;
     const uint64_t last = first + stripe < rows ? first + stripe : rows;
-    for (uint64_t r = first + threadIdx.x; r < last; r += 64)
+    for (uint64_t r = first + threadIdx.x; r < last; r += blockDim.x)
         atomicAdd(&count[type_at(types, (uint32_t)r, n_types)], 1);
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t <= n_types; t += 64)
-        counts[(uint64_t)t * stripes + blockIdx.x] = count[t];
+    for (uint32_t t = threadIdx.x; t <= n_types; t += blockDim.x)
+        counts[(uint64_t)t * gridDim.x + blockIdx.x] = count[t];
 }
 
-// counts[type][stripe] -> exclusive sums over the stripes; totals[type]
+// counts[type][stripe] -> sums over the stripes before; totals[type].  A wave per type, kStripes
+// counts at most.
+constexpr uint32_t kStripes = 1024;
 __global__ __launch_bounds__(256) void plan_scan_kernel(int *__restrict__ counts, uint32_t stripes,
-                                                        int *__restrict__ totals) {
-    __shared__ int wave_sum[4];
-    int *row = counts + (uint64_t)blockIdx.x * stripes;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int carry = 0;
-    for (uint32_t first = 0; first < stripes; first += 256) {
-        const uint32_t i = first + threadIdx.x;
-        const int own = i < stripes ? row[i] : 0;
-        int sum = own;
+                                                        uint32_t groups, int *__restrict__ totals) {
+    constexpr int N = kStripes / 64;
+    const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= groups) return;
+    const int lane = threadIdx.x & 63;
+    int *row = counts + (uint64_t)t * stripes, own[N], carry = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) own[i] = 64u * i + lane < stripes ? row[64 * i + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (64u * i >= stripes) break;
+        int sum = own[i];
         for (int step = 1; step < 64; step <<= 1) {
             const int other = __shfl_up(sum, step);
             if (lane >= step) sum += other;
         }
-        if (lane == 63) wave_sum[wave] = sum;
-        __syncthreads();
-        int before = carry;
-        for (int w = 0; w < wave; ++w) before += wave_sum[w];
-        if (i < stripes) row[i] = before + sum - own;
-        carry += wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
-        __syncthreads();
+        if (64u * i + lane < stripes) row[64 * i + lane] = carry + sum - own[i];
+        carry += __shfl(sum, 63);
     }
-    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+    if (lane == 0) totals[t] = carry;
 }
 
-// Pieces of at most `piece` consecutive positions of one type, as (type, first position), -1 behind
-// the last; first[t] = pieces before type t.  With `totals` the offsets are made from them first.
-// One workgroup; `groups` = the types and, for a plan's tiles, the unknown rows.
-__global__ __launch_bounds__(1024) void plan_pieces_kernel(const int *__restrict__ totals, int *offsets,
-                                                           uint32_t groups, uint32_t piece,
-                                                           uint32_t bound, int2 *__restrict__ pieces,
-                                                           int *__restrict__ first) {
-    __shared__ int sums[2][16];
-    __shared__ int carry[2];
+// LDS: next[waves][n_types + 1].
+template <typename I>
+__global__ __launch_bounds__(256) void plan_place_kernel(const I *__restrict__ types, PlanView p,
+                                                         uint32_t stripe, uint32_t stripes,
+                                                         const int *__restrict__ counts, int bits,
+                                                         const int *__restrict__ totals) {
+    extern __shared__ int next[];
+    __shared__ int sums[2][4];
+    const uint32_t groups = p.types + 1, threads = blockDim.x, waves = threads >> 6;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x < 2) carry[threadIdx.x] = 0;
+    for (uint32_t t = threadIdx.x; t < groups * waves; t += threads) next[t] = 0;
     __syncthreads();
-    for (uint32_t base = 0; base < groups; base += 1024) {
+    // the rows of the waves' own parts of the stripe
+    const uint64_t first = (uint64_t)blockIdx.x * stripe;
+    const uint64_t last = first + stripe < p.rows ? first + stripe : p.rows;
+    const uint32_t part = ((stripe + waves - 1) / waves + 63) / 64 * 64;
+    const uint64_t from = min(first + (uint64_t)wave * part, last), to = min(from + part, last);
+    if (waves > 1)
+        for (uint64_t r = from + lane; r < to; r += 64)
+            atomicAdd(&next[wave * groups + type_at(types, (uint32_t)r, p.types)], 1);
+    __syncthreads();
+    int carry = 0, carry_tiles = 0;
+    for (uint32_t base = 0; base < groups; base += threads) {
         const uint32_t t = base + threadIdx.x;
-        const int own = t >= groups ? 0 : totals ? totals[t] : offsets[t + 1] - offsets[t];
-        const int own_pieces = (int)(((uint32_t)own + piece - 1) / piece);
-        int rows = own, count = own_pieces;
+        int before = 0, total = 0;
+        if (t < groups) {
+            before = counts[(uint64_t)t * stripes + blockIdx.x];
+            total = totals[t];
+        }
+        const int own_tiles = (int)(((uint32_t)total + kTileRows - 1) / kTileRows);
+        int rows = total, tiles = own_tiles;
         for (int step = 1; step < 64; step <<= 1) {
-            const int a = __shfl_up(rows, step), b = __shfl_up(count, step);
+            const int a = __shfl_up(rows, step), b = __shfl_up(tiles, step);
             if (lane >= step) {
                 rows += a;
-                count += b;
+                tiles += b;
             }
         }
         if (lane == 63) {
             sums[0][wave] = rows;
-            sums[1][wave] = count;
+            sums[1][wave] = tiles;
         }
         __syncthreads();
-        int before = carry[0], before_pieces = carry[1];
-        for (int w = 0; w < wave; ++w) {
-            before += sums[0][w];
-            before_pieces += sums[1][w];
-        }
-        const int start = before + rows - own, at = before_pieces + count - own_pieces;
-        if (t < groups) {
-            if (totals) offsets[t] = start;
-            if (first) first[t] = at;
-        }
-        const int from = totals ? start : (t < groups ? offsets[t] : 0);
-        // a wave lists its 64 types one after the other: a type may hold all the pieces
-        for (int l = 0; l < 64; ++l) {
-            const int n = __shfl(own_pieces, l);
-            if (n == 0) continue;
-            const int type = __shfl((int)t, l), f = __shfl(from, l), a = __shfl(at, l);
-            for (int i = lane; i < n; i += 64)
-                pieces[a + i] = make_int2(type, f + (int)((uint32_t)i * piece));
-        }
-        __syncthreads();
-        if (threadIdx.x == 0)
-            for (int w = 0; w < 16; ++w) {
-                carry[0] += sums[0][w];
-                carry[1] += sums[1][w];
+        int start = carry + rows - total, start_tiles = carry_tiles + tiles - own_tiles;
+        for (uint32_t w = 0; w < waves; ++w) {
+            if ((int)w < wave) {
+                start += sums[0][w];
+                start_tiles += sums[1][w];
             }
+            carry += sums[0][w];
+            carry_tiles += sums[1][w];
+        }
+        if (t < groups) {
+            if (blockIdx.x == 0) {
+                p.offsets[t] = start;
+                p.tile_first[t] = start_tiles;
+            }
+            int at = start + before;
+            for (uint32_t w = 0; w < waves; ++w) {
+                const int own = next[w * groups + t];
+                next[w * groups + t] = at;
+                at += own;
+            }
+        }
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        if (totals) offsets[groups] = carry[0];
-        if (first) first[groups] = carry[1];
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.offsets[groups] = carry;
+        p.tile_first[groups] = carry_tiles;
     }
-    for (uint32_t i = (uint32_t)carry[1] + threadIdx.x; i < bound; i += 1024)
-        pieces[i] = make_int2(-1, 0);
+    // every wave walks its own part: its counters belong to no other wave
+    volatile int *mine = next + wave * groups;
+    for (uint64_t base = from; base < to; base += 256) {
+        int type4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t r = base + 64 * i + lane;
+            type4[i] = r < to ? type_at(types, (uint32_t)r, p.types) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t r = base + 64 * i + lane;
+            const int type = type4[i];
+            const bool live = r < to;
+            unsigned long long same = __ballot(live);
+            for (int b = 0; b < bits; ++b) {
+                const unsigned long long set = __ballot(type >> b & 1);
+                same &= type >> b & 1 ? set : ~set;
+            }
+            const unsigned long long below = same & ((1ull << lane) - 1);
+            const int at = live ? mine[type] : 0;
+            __builtin_amdgcn_wave_barrier();  // every lane has read its counter
+            if (live) {
+                p.order[at + __popcll(below)] = (int)r;
+                p.row_types[at + __popcll(below)] = type;
+                if (below == 0) mine[type] = at + __popcll(same);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
 }
 
-template <typename I>
-__global__ __launch_bounds__(64) void plan_place_kernel(const I *__restrict__ types, PlanView p,
-                                                        uint32_t stripe, uint32_t stripes,
-                                                        const int *__restrict__ counts, int bits) {
-    extern __shared__ int next[];
-    for (uint32_t t = threadIdx.x; t <= p.types; t += 64)
-        next[t] = p.offsets[t] + counts[(uint64_t)t * stripes + blockIdx.x];
-    __syncthreads();
-    const uint64_t first = (uint64_t)blockIdx.x * stripe;
-    const uint64_t last = first + stripe < p.rows ? first + stripe : p.rows;
-    for (uint64_t base = first; base < last; base += 64) {
-        const uint64_t r = base + threadIdx.x;
-        const bool live = r < last;
-        const int type = live ? type_at(types, (uint32_t)r, p.types) : 0;
-        unsigned long long same = __ballot(live);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long set = __ballot(type >> b & 1);
-            same &= type >> b & 1 ? set : ~set;
-        }
-        const unsigned long long below = same & ((1ull << threadIdx.x) - 1);
-        if (live) {
-            const int at = next[type] + __popcll(below);
-            p.order[at] = (int)r;
-            p.row_types[at] = type;
-        }
-        __syncthreads();  // every lane has read its counter
-        if (live && below == 0) next[type] += __popcll(same);
-        __syncthreads();
+// The plan's words at indexes that are uniform in the wave, through the scalar cache: a vector load would
+// have to be waited for together with the rows that are being fetched ahead.
+__device__ __forceinline__ int plan_word(const int *p, int i) {
+    typedef const __attribute__((address_space(4))) int *scalar_ptr;
+    return ((scalar_ptr)(uintptr_t)p)[__builtin_amdgcn_readfirstlane(i)];
+}
+
+// Where a tile lies: its type, first position, and the position behind its type's last row.
+struct TileAt {
+    int type, start, end;
+    __device__ __forceinline__ int count() const { return min(kTileRows, end - start); }
+};
+
+// Tile number `t` (uniform in the wave): 64 lanes look at 64 types at a time.
+__device__ __forceinline__ TileAt find_tile(const PlanView &p, int t, int lane) {
+    int lo = 0, hi = (int)p.types + 1;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+        const int c = __popcll(__ballot(i < hi && p.tile_first[i < hi ? i : lo] <= t));
+        lo += (c - 1) * step;
+        hi = min(lo + step, hi);
     }
+    TileAt at;
+    at.type = __builtin_amdgcn_readfirstlane(lo);
+    at.start = plan_word(p.offsets, at.type) + (t - plan_word(p.tile_first, at.type)) * kTileRows;
+    at.end = plan_word(p.offsets, at.type + 1);
+    return at;
+}
+// the tile behind it: at the end of a type that of the next type with rows
+__device__ __forceinline__ TileAt tile_behind(const PlanView &p, TileAt at) {
+    at.start += kTileRows;
+    if (at.start >= at.end) {
+        at.start = at.end;
+        if (at.start < (int)p.rows) {
+            at.type = plan_word(p.row_types, at.start);
+            at.end = plan_word(p.offsets, at.type + 1);
+        }
+    }
+    return at;
 }
 
 // ------------------------------------------------------------------------------- rows and tiles
@@ -252,19 +298,24 @@ template <> struct Tile<__bf16> {
     static constexpr int kPad = 8;
 };
 
-// 16 bytes of a row, zeros from element `valid` on.  `align`: bytes the row's address is a multiple of.
+// How the 16-byte chunks of a row are loaded, chosen on the host for all rows of an operand: kWhole
+// where every row starts on 16 bytes and its length is a multiple of them, kWords where that holds for 4
+// bytes, kElements (bfloat16) else.
+enum ChunkMode : int { kWhole = 0, kWords = 1, kElements = 2 };
+
+// Elements k .. of a row of `length` elements, zeros behind its end or where the row is not `live`.
+// Loads are masked, never corrected afterwards: nothing here waits for what it loads (kElements does),
+// so that a caller can fetch ahead.
 template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T *p, int valid, int align) {
+__device__ __forceinline__ u32x4 load_chunk(const T *row, int k, int length, int mode, bool live = true) {
     constexpr int E = Tile<T>::kChunk;
     u32x4 v = {0, 0, 0, 0};
+    if (!live || k >= length) return v;
+    const T *p = row + k;
+    const int valid = length - k;
     if (valid >= E) {
-        if (align == 16) return *reinterpret_cast<const u32x4 *>(p);
-        if (align == 8) {
-            const uint2 a = reinterpret_cast<const uint2 *>(p)[0];
-            const uint2 b = reinterpret_cast<const uint2 *>(p)[1];
-            return u32x4{a.x, a.y, b.x, b.y};
-        }
-        if (align == 4) {
+        if (mode == kWhole) return *reinterpret_cast<const u32x4 *>(p);
+        if (mode == kWords) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const uint32_t *>(p)[i];
             return v;
@@ -309,6 +360,24 @@ __device__ __forceinline__ void store4(__bf16 *p, f32x4 v, int valid, bool vec) 
         if (i < valid) p[i] = h[i];
 }
 
+// eight consecutive output elements, `valid` of them inside the row; `align`: bytes the rows are
+// aligned to
+__device__ __forceinline__ void store8(float *p, const float *v, int valid, int align) {
+    store4(p, f32x4{v[0], v[1], v[2], v[3]}, valid, align == 16);
+    store4(p + 4, f32x4{v[4], v[5], v[6], v[7]}, valid - 4, align == 16);
+}
+__device__ __forceinline__ void store8(__bf16 *p, const float *v, int valid, int align) {
+    if (align == 16 && valid >= 8) {
+        bf16x8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = to_bf16(v[i]);
+        *reinterpret_cast<bf16x8 *>(p) = h;
+        return;
+    }
+    store4(p, f32x4{v[0], v[1], v[2], v[3]}, valid, align >= 8);
+    store4(p + 4, f32x4{v[4], v[5], v[6], v[7]}, valid - 4, align >= 8);
+}
+
 __device__ __forceinline__ bf16x4 read_transposed(const __bf16 *p) {
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
     const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p));
@@ -316,6 +385,15 @@ __device__ __forceinline__ bf16x4 read_transposed(const __bf16 *p) {
 }
 __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) {
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Tiles dealt out evenly, in order, to at most as many ranges as there are tiles, so that none is empty:
+// the first tile of range r, the range of tile t.
+__device__ __forceinline__ int range_first(uint32_t r, int tiles, uint32_t ranges) {
+    return (int)((uint64_t)r * (uint32_t)tiles / ranges);
+}
+__device__ __forceinline__ int range_of(int t, int tiles, uint32_t ranges) {
+    return (int)(((uint64_t)(t + 1) * ranges - 1) / (uint32_t)tiles);
 }
 
 // The 16 outer x kSlab inner operand fragment of a wave.  Inner elements are dealt to the lanes in an
@@ -328,6 +406,9 @@ template <> struct Frag<float> {
     __device__ __forceinline__ void rows(const float *s, int stride, int outer, int inner, int lane) {
         v = *reinterpret_cast<const f32x4 *>(s + (outer + (lane & 15)) * stride + inner + 4 * (lane >> 4));
     }
+    __device__ __forceinline__ void rank_row(const float *s, int stride, int outer, int lane) {
+        rows(s, stride, outer, 0, lane);
+    }
     // rows of outer elements: s[inner][outer]
     __device__ __forceinline__ void columns(const float *s, int stride, int outer, int inner, int lane) {
 #pragma unroll
@@ -335,12 +416,18 @@ template <> struct Frag<float> {
             v[i] = s[(inner + 4 * (lane >> 4) + i) * stride + outer + (lane & 15)];
     }
     __device__ __forceinline__ float sum() const { return (v[0] + v[1]) + (v[2] + v[3]); }
+    __device__ __forceinline__ void clear() { v = f32x4{0.f, 0.f, 0.f, 0.f}; }
 };
 template <> struct Frag<__bf16> {
     bf16x8 v;
     __device__ __forceinline__ void rows(const __bf16 *s, int stride, int outer, int inner, int lane) {
         const __bf16 *p = s + (outer + (lane & 15)) * stride + inner + 4 * (lane >> 4);
         v = join(*reinterpret_cast<const bf16x4 *>(p), *reinterpret_cast<const bf16x4 *>(p + 16));
+    }
+    // 16 inner elements, for the high parts of the other operand and again for its low parts
+    __device__ __forceinline__ void rank_row(const __bf16 *s, int stride, int outer, int lane) {
+        const bf16x4 q = *reinterpret_cast<const bf16x4 *>(s + (outer + (lane & 15)) * stride + 4 * (lane >> 4));
+        v = join(q, q);
     }
     __device__ __forceinline__ void columns(const __bf16 *s, int stride, int outer, int inner, int lane) {
         const int g = lane >> 4, i = lane & 15;
@@ -353,6 +440,7 @@ template <> struct Frag<__bf16> {
         for (int i = 0; i < 8; ++i) s += (float)v[i];
         return s;
     }
+    __device__ __forceinline__ void clear() { v = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0}); }
 };
 __device__ __forceinline__ f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
 #pragma unroll
@@ -368,19 +456,19 @@ __device__ __forceinline__ f32x4 mma(const Frag<__bf16> &a, const Frag<__bf16> &
 struct WeightView {
     const void *data;
     int64_t type, inner, outer;
-    int align;
+    int mode;  // ChunkMode of its contiguous rows
 };
 
 struct ProductArgs {
     const void *x;
     int64_t ldx;
-    int x_align;
+    int x_mode;
     WeightView w;
     const void *bias;  // [type][N] or [N] (adapted form), may be NULL
     int64_t bias_type;
     void *y;           // rows at their ids; `sorted`: float32 rows at their positions
     int64_t ldy;
-    int y_vec, sorted;
+    int y_align, sorted;
     float scale;       // of the product (before the bias)
     PlanView plan;
     int K, N;
@@ -388,6 +476,11 @@ struct ProductArgs {
     const float *low;
     int rank;
     WeightView up;
+    // narrow_product_kernel, adapted form: x down, times `scale`, is made on the way and kept in
+    // low_out[position][rank] where that is not NULL
+    WeightView down;
+    float *low_out;
+    uint32_t ranges;  // workgroups that share the tiles
 };
 
 // 8 XCDs, each with an L2 of its own, take workgroups in turn: the column blocks of a tile follow one
@@ -416,7 +509,7 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
     __shared__ __align__(16) T ws[WT ? BN * XS : BK * WS];
     __shared__ int ids[64], types[64];
     uint32_t tile, column;
-    const uint32_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : a.plan.tile_bound;
+    const uint32_t tiles = ADAPT ? (a.plan.rows + 63) / 64 : (uint32_t)plan_word(a.plan.tile_first, (int)a.plan.types + 1);
     if (!tile_of_block(tiles, (uint32_t)((a.N + BN - 1) / BN), &tile, &column)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n0 = (int)column * BN;
@@ -425,11 +518,10 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
         start = (int)(tile * 64);
         count = min(64, (int)(a.plan.rows - tile * 64));
     } else {
-        const int2 t = a.plan.tiles[tile];
-        type = t.x;
-        start = t.y;
-        if (type < 0) return;
-        count = min(64, a.plan.offsets[type + 1] - start);
+        const TileAt at = find_tile(a.plan, (int)tile, lane);
+        type = at.type;
+        start = at.start;
+        count = at.count();
     }
     if (tid < 64) {
         ids[tid] = tid < count ? a.plan.order[start + tid] : 0;
@@ -447,9 +539,8 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
 #pragma unroll
             for (int i = 0; i < XL; ++i) {
                 const int c = tid + 256 * i, row = c / (BK / E), k = k0 + c % (BK / E) * E;
-                xr[i] = row < count
-                            ? load_chunk((const T *)a.x + (int64_t)ids[row] * a.ldx + k, a.K - k, a.x_align)
-                            : u32x4{0, 0, 0, 0};
+                // rows behind the tile's last stand for row 0: nobody stores what they give
+                xr[i] = load_chunk((const T *)a.x + (int64_t)ids[row] * a.ldx, k, a.K, a.x_mode);
             }
         };
         auto fetch_w = [&](const T *p, const WeightView &v, int k0, int depth) {
@@ -458,12 +549,11 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
                 const int c = tid + 256 * i;
                 if (WT) {
                     const int n = c / (BK / E), k = k0 + c % (BK / E) * E;
-                    wr[i] = n0 + n < a.N ? load_chunk(p + (int64_t)(n0 + n) * v.outer + k, depth - k, v.align)
-                                         : u32x4{0, 0, 0, 0};
+                    // columns behind the last one likewise
+                    wr[i] = load_chunk(p + (int64_t)min(n0 + n, a.N - 1) * v.outer, k, depth, v.mode);
                 } else {
                     const int k = k0 + c / (BN / E), n = n0 + c % (BN / E) * E;
-                    wr[i] = k < depth ? load_chunk(p + (int64_t)k * v.inner + n, a.N - n, v.align)
-                                      : u32x4{0, 0, 0, 0};
+                    wr[i] = load_chunk(p + (int64_t)k * v.inner, n, a.N, v.mode, k < depth);
                 }
             }
         };
@@ -597,10 +687,269 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
             if (row >= count) continue;
             const f32x4 v = acc[mi][ni] * a.scale + bias;
             if (a.sorted)
-                store4((float *)a.y + (int64_t)(start + row) * a.ldy + n, v, a.N - n, a.y_vec);
+                store4((float *)a.y + (int64_t)(start + row) * a.ldy + n, v, a.N - n, a.y_align == 16);
             else
-                store4((T *)a.y + (int64_t)ids[row] * a.ldy + n, v, a.N - n, a.y_vec);
+                store4((T *)a.y + (int64_t)ids[row] * a.ldy + n, v, a.N - n, a.y_align >= (int)(4 * sizeof(T)));
         }
+    }
+}
+
+// ------------------------------------------------------------------------- rows of some hundred bytes
+// The same product where a row's inner elements fit one LDS tile (128 floats, 256 bfloat16 elements):
+// what an embedding table has.  A workgroup of eight waves takes consecutive tiles of the plan, keeps the
+// weights of the current type in its registers -- 16 columns per wave -- and has the next tile's rows
+// under way while it multiplies.  ADAPT: the weights are shared and stay for the whole launch; a tile's
+// low-rank rows x A are made from the tile itself (one more MFMA column block), go through LDS and are
+// multiplied by B as one more step: x is read once.
+//
+// What a CU can have under way towards its L2 bounds both the rows and the weights (some 20 KB a
+// microsecond): weights are therefore read once per workgroup, whole lines at a time, and dealt out
+// through the LDS of the rows.
+constexpr int kFusedRank = 16;
+constexpr int kNarrowThreads = 512;
+
+// Rows multiplied at a time: half a tile where LDS would else hold one workgroup per CU.
+constexpr int narrow_rows(int slabs, bool adapt) { return slabs == 8 && adapt ? 32 : 64; }
+
+// 16-column blocks per wave.  Two, whose columns a lane holds in turn, make the stores of a bfloat16 row
+// 64 bytes long instead of 32 (a launch of 2.4 M rows of 128: 250 us instead of 299); longer rows leave
+// no registers for it, and float rows need no help.
+constexpr int narrow_blocks(int size, int slabs) { return size == 2 && slabs < 8 ? 2 : 1; }
+
+template <typename T, int SLABS, int BN, bool WT, bool ADAPT>
+__global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(ProductArgs a) {
+    constexpr int E = Tile<T>::kChunk, SLAB = Tile<T>::kSlab, DEPTH = SLABS * SLAB;
+    constexpr int XS = DEPTH + Tile<T>::kPad, CHUNKS = DEPTH / E;
+    constexpr int NI = narrow_blocks(sizeof(T), SLABS), WAVES_N = BN / (16 * NI), WAVES_M = 8 / WAVES_N;
+    constexpr int ROWS = narrow_rows(SLABS, ADAPT), MI = ROWS / 16 / WAVES_M;
+    constexpr int XL = ROWS * CHUNKS / kNarrowThreads;
+    static_assert(MI >= 1 && XL >= 1, "every wave has rows, every thread a chunk");
+    constexpr int LS = sizeof(T) == 4 ? 20 : 40;  // low-rank rows in LDS: 16 floats, or 16 + 16 halves
+    // the weights' way through LDS: STEP slabs at a time, inner elements or columns as rows
+    constexpr int WS = BN + (sizeof(T) == 4 ? 4 : 16);
+    constexpr int LDS_X = 2 * ROWS * XS, LDS_W = LDS_X > 17408 / (int)sizeof(T) ? LDS_X : 17408 / (int)sizeof(T);
+    constexpr int FIT = LDS_W / (WT ? BN * (SLAB + Tile<T>::kPad) : SLAB * WS);
+    constexpr int STEP = FIT >= SLABS ? SLABS : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+    constexpr int WTS = STEP * SLAB + Tile<T>::kPad;
+    static_assert((WT ? BN * WTS : STEP * SLAB * WS) <= LDS_W || STEP == 1, "weights in passes");
+    __shared__ __align__(16) T xs[LDS_W];
+    __shared__ __align__(16) T ls[ADAPT ? ROWS * LS : 1];
+    __shared__ __align__(16) T as[ADAPT ? 16 * XS : 1];
+    __shared__ __align__(16) T us[ADAPT ? BN * 20 : 1];  // rows of 16 rank elements and a gap
+    __shared__ int ids[3][64];
+    uint32_t range, column;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (!tile_of_block(a.ranges, (uint32_t)((a.N + BN - 1) / BN), &range, &column)) return;
+    const int tiles = plan_word(a.plan.tile_first, (int)a.plan.types + 1);
+    const uint32_t ranges = min(a.ranges, (uint32_t)tiles);
+    if (range >= ranges) return;
+    const int first = range_first(range, tiles, ranges), last = range_first(range + 1, tiles, ranges);
+    const int wn = wave % WAVES_N, m0 = wave / WAVES_N * MI * 16, nb = (int)column * BN, n0 = nb + wn * 16 * NI;
+    const int n = n0 + 4 * NI * (lane >> 4);  // the lane's 4 * NI output columns
+    const int unknown = (int)a.plan.types;
+    u32x4 xr[XL];
+    auto fetch = [&](const int *id) {  // ids behind a tile's last row are 0: nobody stores what they give
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int c = tid + kNarrowThreads * i;
+            xr[i] = load_chunk((const T *)a.x + (int64_t)id[c / CHUNKS] * a.ldx, c % CHUNKS * E, a.K, a.x_mode);
+        }
+    };
+    Frag<T> wf[SLABS][NI];
+    // The workgroup's columns of one type's weights, STEP slabs at a time through the rows' LDS; with
+    // two blocks per wave the even columns of 32 go in front of the odd ones.
+    auto load_weights = [&](const T *w) {
+#pragma unroll
+        for (int s0 = 0; s0 < SLABS; s0 += STEP) {
+            if (s0 * SLAB >= a.K) {
+#pragma unroll
+                for (int s = s0; s < s0 + STEP; ++s)
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) wf[s][ni].clear();
+                continue;
+            }
+            constexpr int LINE = WT ? STEP * SLAB / E : BN / E, COUNT = WT ? BN * LINE : STEP * SLAB * LINE;
+            __syncthreads();  // the rows have been multiplied, or the last pass has been read
+#pragma unroll 8
+            for (int c = tid; c < COUNT; c += kNarrowThreads) {
+                const int line = c / LINE, at = c % LINE * E;
+                u32x4 q;
+                if (WT)
+                    q = load_chunk(w + (int64_t)min(nb + line, a.N - 1) * a.w.outer, s0 * SLAB + at, a.K, a.w.mode);
+                else
+                    q = load_chunk(w + (int64_t)(s0 * SLAB + line) * a.w.inner, nb + at, a.N, a.w.mode,
+                                   s0 * SLAB + line < a.K);
+                if constexpr (NI == 2 && WT) {
+                    const int to = (line & ~31) + (line & 1) * 16 + (line & 31) / 2;
+                    *reinterpret_cast<u32x4 *>(xs + to * WTS + at) = q;
+                } else if constexpr (NI == 2) {
+                    T *to = xs + line * WS + (at & ~31) + (at & 31) / 2;
+                    const uint2 even = {(q[0] & 0xFFFFu) | q[1] << 16, (q[2] & 0xFFFFu) | q[3] << 16};
+                    const uint2 odd = {q[0] >> 16 | (q[1] & 0xFFFF0000u), q[2] >> 16 | (q[3] & 0xFFFF0000u)};
+                    *reinterpret_cast<uint2 *>(to) = even;
+                    *reinterpret_cast<uint2 *>(to + 16) = odd;
+                } else {
+                    *reinterpret_cast<u32x4 *>(xs + line * (WT ? WTS : WS) + at) = q;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < STEP; ++s)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) {
+                    if (WT)
+                        wf[s0 + s][ni].rows(xs, WTS, (wn * NI + ni) * 16, s * SLAB, lane);
+                    else
+                        wf[s0 + s][ni].columns(xs, WS, (wn * NI + ni) * 16, s * SLAB, lane);
+                }
+        }
+        __syncthreads();
+    };
+    float bias[4 * NI] = {};
+    auto load_bias = [&](const T *b) {
+        if (!a.bias) return;
+#pragma unroll
+        for (int i = 0; i < 4 * NI; ++i) bias[i] = (float)b[min(n + i, a.N - 1)];
+    };
+    auto id_of = [&](const TileAt &at) { return tid < at.count() ? a.plan.order[at.start + tid] : 0; };
+    TileAt at = find_tile(a.plan, first, lane), ahead = at, ahead2;
+    if (first + 1 < last) ahead = tile_behind(a.plan, at);
+    ahead2 = ahead;
+    if (first + 2 < last) ahead2 = tile_behind(a.plan, ahead);
+    if (tid < 64) {
+        ids[0][tid] = id_of(at);
+        ids[1][tid] = id_of(ahead);
+    }
+    __syncthreads();
+    int loaded = -1;
+    fetch(ids[0]);
+    if (ADAPT) {
+        load_bias((const T *)a.bias);
+        load_weights((const T *)a.w.data);
+    }
+    int slot = 0, buffer = 0;
+    for (int t = first; t < last; ++t) {
+        const bool known = at.type != unknown;
+        if (at.type != loaded && known) {
+            loaded = at.type;
+            if (!ADAPT) {
+                load_bias((const T *)a.bias + (int64_t)at.type * a.bias_type);
+                load_weights((const T *)a.w.data + (int64_t)at.type * a.w.type);
+            } else {
+                // A and B in LDS, their rank elements as rows and within rows, B's columns in the order of
+                // the weights'
+                const T *down = (const T *)a.down.data + (int64_t)at.type * a.down.type;
+                const T *up = (const T *)a.up.data + (int64_t)at.type * a.up.type;
+                __syncthreads();  // the last tile has been multiplied
+#pragma unroll 4
+                for (int i = tid; i < 16 * DEPTH; i += kNarrowThreads) {
+                    const int j = WT ? i / DEPTH : i & 15, k = WT ? i % DEPTH : i >> 4;
+                    const T q = down[min(k, a.K - 1) * a.down.inner + min(j, a.rank - 1) * a.down.outer];
+                    as[j * XS + k] = k < a.K && j < a.rank ? q : (T)0.f;
+                }
+#pragma unroll 4
+                for (int i = tid; i < 16 * BN; i += kNarrowThreads) {
+                    const int j = WT ? i & 15 : i / BN, c = WT ? i >> 4 : i % BN;
+                    const T q = up[min(j, a.rank - 1) * a.up.inner + min(nb + c, a.N - 1) * a.up.outer];
+                    const int to = NI == 2 ? (c & ~31) + (c & 1) * 16 + (c & 31) / 2 : c;
+                    us[to * 20 + j] = j < a.rank ? q : (T)0.f;
+                }
+            }
+        }
+        const int count = at.count(), start = at.start;
+        const int *id = ids[slot];
+        const int next = slot == 2 ? 0 : slot + 1, free = next == 2 ? 0 : next + 1;
+        at = ahead;
+        for (int r0 = 0; r0 < count; r0 += ROWS) {
+            T *x = xs + buffer * ROWS * XS;  // its last readers are behind the last barrier
+            buffer ^= 1;
+#pragma unroll
+            for (int i = 0; i < XL; ++i) {
+                const int c = tid + kNarrowThreads * i;
+                *reinterpret_cast<u32x4 *>(x + c / CHUNKS * XS + c % CHUNKS * E) = xr[i];
+            }
+            __syncthreads();
+            // the ids of the tile behind the next, the next rows: of this tile or of the next one
+            const bool ends = r0 + ROWS >= count;
+            int id_ahead = 0;
+            if (ends && t + 2 < last && tid < 64) id_ahead = id_of(ahead2);
+            if (!ends || t + 1 < last) fetch(ends ? ids[next] : id + r0 + ROWS);
+            // 16-row blocks of this wave that hold rows
+            const int live = (count - r0 - m0 + 15) >> 4;
+            f32x4 acc[MI][NI] = {};
+            if (ADAPT || known) {
+#pragma unroll
+                for (int s = 0; s < SLABS; ++s)
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+                        if (mi < live) {
+                            Frag<T> xf;
+                            xf.rows(x, XS, m0 + mi * 16, s * SLAB, lane);
+#pragma unroll
+                            for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma(wf[s][ni], xf, acc[mi][ni]);
+                        }
+                if (ADAPT && known) {
+                    if (wave * 16 < ROWS && r0 + wave * 16 < count) {
+                        // row block `wave`; lane: rank columns 4 (lane / 16) .. + 3 of row lane % 16
+                        f32x4 low = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int s = 0; s < SLABS; ++s) {
+                            Frag<T> xf, af;
+                            xf.rows(x, XS, wave * 16, s * SLAB, lane);
+                            af.rows(as, XS, 0, s * SLAB, lane);
+                            low = mma(af, xf, low);
+                        }
+                        const int row = wave * 16 + (lane & 15), j = 4 * (lane >> 4);
+                        low *= a.scale;
+                        if (a.low_out && column == 0 && r0 + row < count)
+                            store4(a.low_out + (int64_t)(start + r0 + row) * a.rank + j, low, a.rank - j,
+                                   (a.rank & 3) == 0);
+                        if constexpr (sizeof(T) == 4) {
+                            *reinterpret_cast<f32x4 *>(ls + row * LS + j) = low;
+                        } else {
+                            bf16x4 high, rest;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                high[i] = to_bf16(low[i]);
+                                rest[i] = to_bf16(low[i] - (float)high[i]);
+                            }
+                            *reinterpret_cast<bf16x4 *>(ls + row * LS + j) = high;
+                            *reinterpret_cast<bf16x4 *>(ls + row * LS + 16 + j) = rest;
+                        }
+                    }
+                    __syncthreads();
+                    Frag<T> uf[NI];
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) uf[ni].rank_row(us, 20, (wn * NI + ni) * 16, lane);
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+                        if (mi < live) {
+                            Frag<T> lf;
+                            lf.rows(ls, LS, m0 + mi * 16, 0, lane);
+#pragma unroll
+                            for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma(uf[ni], lf, acc[mi][ni]);
+                        }
+                }
+            }
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) {
+                const int row = r0 + m0 + mi * 16 + (lane & 15);
+                if (row >= count) continue;
+                T *y = (T *)a.y + (int64_t)id[row] * a.ldy + n;
+                float v[4 * NI];
+#pragma unroll
+                for (int i = 0; i < 4 * NI; ++i)
+                    v[i] = ADAPT || known ? acc[mi][i % NI][i / NI] + bias[i] : 0.f;
+                if constexpr (NI == 2)
+                    store8(y, v, a.N - n, a.y_align);
+                else
+                    store4(y, f32x4{v[0], v[1], v[2], v[3]}, a.N - n, a.y_align >= (int)(4 * sizeof(T)));
+            }
+            if (ends && tid < 64) ids[free][tid] = id_ahead;
+        }
+        slot = next;
+        ahead = ahead2;
+        if (t + 3 < last) ahead2 = tile_behind(a.plan, ahead2);
     }
 }
 
@@ -654,7 +1003,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs a) {
     auto accumulate = [&](const T *w, const WeightView &v, const float *vec, int depth) {
 #pragma unroll 8
         for (int k = split; k < depth; k += SPLIT) {
-            const u32x4 q = load_chunk(w + (int64_t)k * v.inner + n0 + c, a.N - n0 - c, v.align);
+            const u32x4 q = load_chunk(w + (int64_t)k * v.inner, n0 + c, a.N, v.mode);
             const float f = vec[k];
 #pragma unroll
             for (int i = 0; i < E; ++i)
@@ -697,29 +1046,39 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs a) {
 }
 
 // ------------------------------------------------------------------------- weights' gradients
-// dW[t] = sum over the rows of type t of x[r]^T dy[r].  The row axis is cut into chunks; a workgroup
-// adds one chunk's outer products of a block of dW in registers, a second launch joins the chunks of
-// a type in their order (no atomics: the same bits in every run).  A type of one chunk is written at
-// once.  Either operand may be float32 rows at their positions (the low-rank rows), which enter
-// bfloat16 products as a high and a low part.
+// dW[t] = sum over the rows of type t of x[r]^T dy[r].  The tiles of the plan are dealt out evenly, in
+// order, to `ranges` workgroups per block of dW; a workgroup adds the outer products of one type's rows
+// in registers.  A type whose tiles lie in one range is written at once.  A range leaves the sums of
+// a type that began before it in its first slot, those of a type that goes on behind it in its second; a
+// second launch joins them in order (no atomics: the same bits in every run).  Either operand may be
+// float32 rows at their positions (the low-rank rows), which enter bfloat16 products as a high and a
+// low part.
 struct GradArgs {
     const void *x, *dy;
     int64_t ldx, ldy;
-    int x_align, y_align;
-    const int *order;    // NULL: rows at their positions
-    const int2 *chunks;  // NULL: one group of all rows
-    const int *first, *offsets;
-    uint32_t rows, types, chunk_rows, chunk_bound;
+    int x_mode, y_mode;
+    PlanView plan;
+    int shared;      // one group: 64 rows after the other, whatever their types
+    uint32_t types;  // of the gradient: 1 if shared
+    uint32_t ranges;
     int K, N;
-    float *partial;  // [chunk][stride]: K * N products, then N column sums
+    float *partial;  // [range][2][stride]: K * N products, then N column sums
     int64_t stride;
     void *dw;        // [type][K][N], may be NULL when only the bias is asked for (K = 0)
     void *db;        // [type][N] or NULL
 };
+__device__ __forceinline__ int grad_tiles(const GradArgs &a) {  // the known types' tiles
+    return a.shared ? (int)((a.plan.rows + kTileRows - 1) / kTileRows)
+                    : plan_word(a.plan.tile_first, (int)a.plan.types);
+}
+
+// waves per SIMD that the registers of a block's sums leave room for
+constexpr int grad_waves(int mi, int ni) { return mi * ni >= 8 ? 2 : 4; }
 
 template <typename T, int MI, int NI, bool XLOW, bool YLOW>
-__global__ __launch_bounds__(256) void grad_kernel(GradArgs a) {
+__global__ __launch_bounds__(256, grad_waves(MI, NI)) void grad_kernel(GradArgs a) {
     constexpr int E = Tile<T>::kChunk, R = Tile<T>::kDepth, STEP = Tile<T>::kSlab;
+    constexpr int STAGES = kTileRows / R;  // a tile is one stage (bfloat16) or two (float)
     constexpr int BM = 32 * MI, BN = 32 * NI;
     constexpr bool SPLITX = XLOW && sizeof(T) == 2, SPLITY = YLOW && sizeof(T) == 2;
     // row strides that keep the four lane groups, four rows apart, in different banks: 4 words more
@@ -728,37 +1087,26 @@ __global__ __launch_bounds__(256) void grad_kernel(GradArgs a) {
     constexpr int XW = BM * (SPLITX ? 2 : 1) + PAD, YW = BN * (SPLITY ? 2 : 1) + PAD;
     constexpr int XL = R * BM / E / 256, YL = R * BN / E / 256;
     static_assert(XL >= 1 && YL >= 1, "a block of at least 32 x 32");
-    __shared__ __align__(16) T xs[R * XW];
-    __shared__ __align__(16) T ys[R * YW];
-    __shared__ int ids[2][R];
+    __shared__ __align__(16) T xss[2][R * XW];
+    __shared__ __align__(16) T yss[2][R * YW];
+    __shared__ int ids[3][kTileRows];
     const uint32_t kb = a.K > 0 ? (uint32_t)((a.K + BM - 1) / BM) : 1, nb = (uint32_t)((a.N + BN - 1) / BN);
-    uint32_t chunk, block;
-    if (!tile_of_block(a.chunk_bound, kb * nb, &chunk, &block)) return;
+    uint32_t range, block;
+    if (!tile_of_block(a.ranges, kb * nb, &range, &block)) return;
     const int k0 = (int)(block / nb) * BM, n0 = (int)(block % nb) * BN;
-    int type = 0, start, last, chunks;
-    if (a.chunks) {
-        const int2 c = a.chunks[chunk];
-        type = c.x;
-        if (type < 0) return;
-        start = c.y;
-        last = a.offsets[type + 1];
-        chunks = a.first[type + 1] - a.first[type];
-    } else {
-        start = (int)(chunk * a.chunk_rows);
-        last = (int)a.rows;
-        chunks = (int)a.chunk_bound;
-    }
-    last = last - start < (int)a.chunk_rows ? last : start + (int)a.chunk_rows;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tiles = grad_tiles(a);
+    const uint32_t ranges = min(a.ranges, (uint32_t)tiles);
+    if (range >= ranges) return;
+    const int first = range_first(range, tiles, ranges), last = range_first(range + 1, tiles, ranges);
     const int wm = wave >> 1, wn = wave & 1;
     f32x4 acc[MI][NI] = {};
     float sums[NI] = {};
     const bool want_sums = a.db && k0 == 0 && wm == 0;
-    auto fetch_id = [&](int p) { return p < last ? (a.order ? a.order[p] : p) : 0; };
     u32x4 xr[XL], yr[YL], xr2[SPLITX ? XL : 1], yr2[SPLITY ? YL : 1];
     // float32 rows in a bfloat16 product: 8 floats -> 8 high and 8 low parts
-    auto fetch_low = [&](const float *p, int valid, int align, u32x4 &high, u32x4 &low) {
-        const u32x4 q0 = load_chunk(p, valid, align), q1 = load_chunk(p + 4, valid - 4, align);
+    auto fetch_low = [&](const float *row, int k, int length, int mode, bool live, u32x4 &high, u32x4 &low) {
+        const u32x4 q0 = load_chunk(row, k, length, mode, live), q1 = load_chunk(row, k + 4, length, mode, live);
         bf16x8 h, l;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -769,148 +1117,187 @@ __global__ __launch_bounds__(256) void grad_kernel(GradArgs a) {
         high = __builtin_bit_cast(u32x4, h);
         low = __builtin_bit_cast(u32x4, l);
     };
-    auto fetch = [&](int p0, const int *id) {
+    // rows r0 .. of a tile, `id` = its ids; rows behind its last count as zeros
+    auto fetch = [&](const TileAt &at, const int *id, int r0) {
+        const int count = at.count();
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
-            const int c = tid + 256 * i, row = c / (BM / E), k = k0 + c % (BM / E) * E;
-            const bool live = p0 + row < last && k < a.K;
-            xr[i] = u32x4{0, 0, 0, 0};
-            if constexpr (SPLITX) {
-                xr2[i] = u32x4{0, 0, 0, 0};
-                if (live)
-                    fetch_low((const float *)a.x + (int64_t)(p0 + row) * a.ldx + k, a.K - k, a.x_align, xr[i], xr2[i]);
-            } else if (live) {
-                xr[i] = load_chunk((const T *)a.x + (int64_t)(XLOW ? p0 + row : id[row]) * a.ldx + k, a.K - k, a.x_align);
-            }
+            const int c = tid + 256 * i, row = r0 + c / (BM / E), k = k0 + c % (BM / E) * E;
+            const int64_t r = XLOW ? at.start + row : id[row];
+            if constexpr (SPLITX)
+                fetch_low((const float *)a.x + r * a.ldx, k, a.K, a.x_mode, row < count, xr[i], xr2[i]);
+            else
+                xr[i] = load_chunk((const T *)a.x + r * a.ldx, k, a.K, a.x_mode, row < count);
         }
 #pragma unroll
         for (int i = 0; i < YL; ++i) {
-            const int c = tid + 256 * i, row = c / (BN / E), n = n0 + c % (BN / E) * E;
-            const bool live = p0 + row < last && n < a.N;
-            yr[i] = u32x4{0, 0, 0, 0};
-            if constexpr (SPLITY) {
-                yr2[i] = u32x4{0, 0, 0, 0};
-                if (live)
-                    fetch_low((const float *)a.dy + (int64_t)(p0 + row) * a.ldy + n, a.N - n, a.y_align, yr[i], yr2[i]);
-            } else if (live) {
-                yr[i] = load_chunk((const T *)a.dy + (int64_t)(YLOW ? p0 + row : id[row]) * a.ldy + n, a.N - n, a.y_align);
-            }
+            const int c = tid + 256 * i, row = r0 + c / (BN / E), n = n0 + c % (BN / E) * E;
+            const int64_t r = YLOW ? at.start + row : id[row];
+            if constexpr (SPLITY)
+                fetch_low((const float *)a.dy + r * a.ldy, n, a.N, a.y_mode, row < count, yr[i], yr2[i]);
+            else
+                yr[i] = load_chunk((const T *)a.dy + r * a.ldy, n, a.N, a.y_mode, row < count);
         }
     };
-    if (tid < R) {
-        ids[0][tid] = fetch_id(start + tid);
-        ids[1][tid] = fetch_id(start + R + tid);
+    auto id_at = [&](const TileAt &at) {
+        return tid >= at.count() ? 0 : a.shared ? at.start + tid : a.plan.order[at.start + tid];
+    };
+    auto behind = [&](TileAt at) {
+        if (!a.shared) return tile_behind(a.plan, at);
+        at.start += kTileRows;
+        return at;
+    };
+    TileAt at;
+    if (a.shared) {
+        at.type = 0;
+        at.start = first * kTileRows;
+        at.end = (int)a.plan.rows;
+    } else {
+        at = find_tile(a.plan, first, lane);
+    }
+    TileAt ahead = at, ahead2;
+    if (first + 1 < last) ahead = behind(at);
+    ahead2 = ahead;
+    if (first + 2 < last) ahead2 = behind(ahead);
+    if (tid < kTileRows) {
+        ids[0][tid] = id_at(at);
+        ids[1][tid] = id_at(ahead);
     }
     __syncthreads();
-    fetch(start, ids[0]);
-    int next = 1;
-    for (int p0 = start; p0 < last; p0 += R) {
+    fetch(at, ids[0], 0);
+    int slot = 0, buffer = 0;
+    for (int t = first; t < last; ++t) {
+        const TileAt now = at;
+        const int next = slot == 2 ? 0 : slot + 1, free = next == 2 ? 0 : next + 1;
 #pragma unroll
-        for (int i = 0; i < XL; ++i) {
-            const int c = tid + 256 * i;
-            T *to = xs + c / (BM / E) * XW + c % (BM / E) * E;
-            *reinterpret_cast<u32x4 *>(to) = xr[i];
-            if constexpr (SPLITX) *reinterpret_cast<u32x4 *>(to + BM) = xr2[i];
-        }
+        for (int stage = 0; stage < STAGES; ++stage) {
+            // a wave that writes this buffer has passed the barrier behind its last readers
+            T *xs = xss[buffer], *ys = yss[buffer];
+            buffer ^= 1;
 #pragma unroll
-        for (int i = 0; i < YL; ++i) {
-            const int c = tid + 256 * i;
-            T *to = ys + c / (BN / E) * YW + c % (BN / E) * E;
-            *reinterpret_cast<u32x4 *>(to) = yr[i];
-            if constexpr (SPLITY) *reinterpret_cast<u32x4 *>(to + BN) = yr2[i];
-        }
-        __syncthreads();
-        int ahead = 0;
-        if (p0 + R < last) {
-            fetch(p0 + R, ids[next]);
-            if (tid < R) ahead = fetch_id(p0 + 2 * R + tid);
-        }
-#pragma unroll
-        for (int r = 0; r < R; r += STEP) {
-            Frag<T> yf[NI], yl[SPLITY ? NI : 1];
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-                yf[ni].columns(ys, YW, wn * NI * 16 + ni * 16, r, lane);
-                if constexpr (SPLITY) yl[ni].columns(ys, YW, BN + wn * NI * 16 + ni * 16, r, lane);
-                if (want_sums) sums[ni] += yf[ni].sum();
+            for (int i = 0; i < XL; ++i) {
+                const int c = tid + 256 * i;
+                T *to = xs + c / (BM / E) * XW + c % (BM / E) * E;
+                *reinterpret_cast<u32x4 *>(to) = xr[i];
+                if constexpr (SPLITX) *reinterpret_cast<u32x4 *>(to + BM) = xr2[i];
             }
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) {
-                Frag<T> xf;
-                xf.columns(xs, XW, wm * MI * 16 + mi * 16, r, lane);
+            for (int i = 0; i < YL; ++i) {
+                const int c = tid + 256 * i;
+                T *to = ys + c / (BN / E) * YW + c % (BN / E) * E;
+                *reinterpret_cast<u32x4 *>(to) = yr[i];
+                if constexpr (SPLITY) *reinterpret_cast<u32x4 *>(to + BN) = yr2[i];
+            }
+            __syncthreads();
+            // the ids of the tile behind the next, the next rows: of this tile or of the next one
+            const bool ends = stage + 1 == STAGES;
+            int id_ahead = 0;
+            if (ends && t + 2 < last && tid < kTileRows) id_ahead = id_at(ahead2);
+            if (!ends || t + 1 < last) fetch(ends ? ahead : now, ids[ends ? next : slot], ends ? 0 : R * (stage + 1));
+#pragma unroll
+            for (int r = 0; r < R; r += STEP) {
+                Frag<T> yf[NI], yl[SPLITY ? NI : 1];
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni) {
-                    acc[mi][ni] = mma(yf[ni], xf, acc[mi][ni]);
-                    if constexpr (SPLITY) acc[mi][ni] = mma(yl[ni], xf, acc[mi][ni]);
+                    yf[ni].columns(ys, YW, wn * NI * 16 + ni * 16, r, lane);
+                    if constexpr (SPLITY) yl[ni].columns(ys, YW, BN + wn * NI * 16 + ni * 16, r, lane);
+                    if (want_sums) sums[ni] += yf[ni].sum();
                 }
-                if constexpr (SPLITX) {
-                    xf.columns(xs, XW, BM + wm * MI * 16 + mi * 16, r, lane);
 #pragma unroll
-                    for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma(yf[ni], xf, acc[mi][ni]);
+                for (int mi = 0; mi < MI; ++mi) {
+                    Frag<T> xf;
+                    xf.columns(xs, XW, wm * MI * 16 + mi * 16, r, lane);
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) {
+                        acc[mi][ni] = mma(yf[ni], xf, acc[mi][ni]);
+                        if constexpr (SPLITY) acc[mi][ni] = mma(yl[ni], xf, acc[mi][ni]);
+                    }
+                    if constexpr (SPLITX) {
+                        xf.columns(xs, XW, BM + wm * MI * 16 + mi * 16, r, lane);
+#pragma unroll
+                        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma(yf[ni], xf, acc[mi][ni]);
+                    }
                 }
             }
+            if (ends && tid < kTileRows) ids[free][tid] = id_ahead;
         }
-        __syncthreads();
-        next ^= 1;
-        if (tid < R) ids[next][tid] = ahead;  // the ids used last are free: `fetch` of the stage after next
-    }
-    // lane: row k = lane % 16 of the block, four consecutive columns n
-    float *part = a.partial + (int64_t)chunk * a.stride;
+        slot = next;
+        at = ahead;
+        ahead = ahead2;
+        if (t + 3 < last) ahead2 = behind(ahead2);
+        if (t + 1 < last && at.type == now.type) continue;
+        // the type or the range ends here: its sums are whole, or one range's share of them
+        const int type_first = a.shared ? 0 : plan_word(a.plan.tile_first, now.type);
+        const int type_last = a.shared ? tiles : plan_word(a.plan.tile_first, now.type + 1);
+        const bool whole = type_first >= first && type_last <= last;
+        float *part = a.partial + (int64_t)(2 * range + (type_first >= first)) * a.stride;
+        // lane: row k = lane % 16 of the block, four consecutive columns n
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-        const int k = k0 + wm * MI * 16 + mi * 16 + (lane & 15);
-        if (k >= a.K) continue;
+        for (int mi = 0; mi < MI; ++mi) {
+            const int k = k0 + wm * MI * 16 + mi * 16 + (lane & 15);
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni) {
-            const int n = n0 + wn * NI * 16 + ni * 16 + 4 * (lane >> 4);
-            const bool vec = (a.N & 3) == 0;
-            if (chunks == 1)
-                store4((T *)a.dw + ((int64_t)type * a.K + k) * a.N + n, acc[mi][ni], a.N - n, vec);
-            else
-                store4(part + (int64_t)k * a.N + n, acc[mi][ni], a.N - n, vec);
+            for (int ni = 0; ni < NI; ++ni) {
+                const int n = n0 + wn * NI * 16 + ni * 16 + 4 * (lane >> 4);
+                const bool vec = (a.N & 3) == 0;
+                if (k < a.K) {
+                    if (whole)
+                        store4((T *)a.dw + ((int64_t)now.type * a.K + k) * a.N + n, acc[mi][ni], a.N - n, vec);
+                    else
+                        store4(part + (int64_t)k * a.N + n, acc[mi][ni], a.N - n, vec);
+                }
+                acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         }
-    }
-    if (want_sums) {
+        if (want_sums) {
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni) {
-            float s = sums[ni];
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            const int n = n0 + wn * NI * 16 + ni * 16 + lane;
-            if (lane < 16 && n < a.N) {
-                if (chunks == 1)
-                    ((T *)a.db)[(int64_t)type * a.N + n] = (T)s;
-                else
-                    part[(int64_t)a.K * a.N + n] = s;
+            for (int ni = 0; ni < NI; ++ni) {
+                float s = sums[ni];
+                s += __shfl_xor(s, 16);
+                s += __shfl_xor(s, 32);
+                const int n = n0 + wn * NI * 16 + ni * 16 + lane;
+                if (lane < 16 && n < a.N) {
+                    if (whole)
+                        ((T *)a.db)[(int64_t)now.type * a.N + n] = (T)s;
+                    else
+                        part[(int64_t)a.K * a.N + n] = s;
+                }
+                sums[ni] = 0.f;
             }
         }
     }
 }
 
-// Joins the chunks of a type in their order: sixteen waves sum a sixteenth of them each, 256 elements
-// at a time.  Types without rows get zeros; types of one chunk are done.
+// Joins the ranges of a type in their order: the workgroup's waves sum an equal share of them each, 256
+// elements at a time.  Types without rows get zeros; types inside one range are done.
 template <typename T>
 __global__ __launch_bounds__(1024) void grad_join_kernel(GradArgs a) {
     __shared__ f32x4 part[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int64_t blocks = (a.stride + 255) / 256;
     const int type = (int)(blockIdx.x / blocks);
     const int64_t at = (int64_t)(blockIdx.x % blocks) * 256 + lane * 4;
-    const int first = a.chunks ? a.first[type] : 0;
-    const int count = a.chunks ? a.first[type + 1] - first : (int)a.chunk_bound;
-    if (count == 1) return;
-    const int share = (count + 15) / 16;
+    const int tiles = a.plan.rows ? grad_tiles(a) : 0;
+    const int type_first = a.shared || !tiles ? 0 : a.plan.tile_first[type];
+    const int type_last = a.shared || !tiles ? tiles : a.plan.tile_first[type + 1];
+    int first = 0, count = 0;  // the ranges it lies in
+    if (type_last > type_first) {
+        const uint32_t ranges = min(a.ranges, (uint32_t)tiles);
+        first = range_of(type_first, tiles, ranges);
+        count = range_of(type_last - 1, tiles, ranges) - first + 1;
+        if (count == 1) return;
+    }
+    const int share = (count + waves - 1) / waves;
     const int from = first + min(count, wave * share), to = first + min(count, (wave + 1) * share);
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (at < a.stride) {
 #pragma unroll 8
-        for (int c = from; c < to; ++c)
-            sum += *reinterpret_cast<const f32x4 *>(a.partial + (int64_t)c * a.stride + at);
+        for (int r = from; r < to; ++r)  // its first range holds it behind other types
+            sum += *reinterpret_cast<const f32x4 *>(a.partial + (int64_t)(2 * r + (r == first)) * a.stride + at);
     }
     part[wave][lane] = sum;
     __syncthreads();
     if (wave == 0) {
-        for (int w = 1; w < 16; ++w) sum += part[w][lane];
+        for (int w = 1; w < waves; ++w) sum += part[w][lane];
         const int64_t weights = (int64_t)a.K * a.N;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -174,6 +174,23 @@ def _typed_product(x, ldx, weight, plan, outputs, bias=None):
     return y
 
 
+def _adapted_product(x, ldx, weight, down, up, rank, scale, plan, outputs, bias=None, low=None):
+    """``low``: float32 [rows, rank], filled with the low-rank rows at their positions in the plan's
+    order; None where nobody needs them."""
+    torch = _torch()
+    if low is None and (rank > _lib.FUSED_RANK
+                        or x.shape[1] * x.element_size() > _lib.FUSED_ROW_BYTES):
+        low = torch.empty((x.shape[0], rank), dtype=torch.float32, device=x.device)
+    y = torch.empty((x.shape[0], outputs), dtype=x.dtype, device=x.device)
+    io = _product_io(x, ldx, weight, y, x.shape[1], outputs, plan.number_of_types)
+    io.d_plan, io.down, io.up, io.rank, io.scale = plan._words.data_ptr(), down, up, rank, scale
+    if low is not None:
+        io.d_low = low.data_ptr()
+    bias = _set_bias(io, bias)
+    _lib.check(_lib.lib().gn2v_adapted_product(C.byref(io), _stream(x)))
+    return y
+
+
 def _low_rows(x, ldx, weight, plan, rank, scale):
     """scale * x[r] W[type of r] as float32 rows at their positions in the plan's order."""
     low = _torch().empty((x.shape[0], rank), dtype=_torch().float32, device=x.device)
@@ -181,16 +198,6 @@ def _low_rows(x, ldx, weight, plan, rank, scale):
     io.d_plan, io.scale, io.low_rank_rows = plan._words.data_ptr(), scale, 1
     _lib.check(_lib.lib().gn2v_typed_product(C.byref(io), _stream(x)))
     return low
-
-
-def _adapted_product(x, ldx, weight, up, low, plan, outputs, bias=None):
-    y = _torch().empty((x.shape[0], outputs), dtype=x.dtype, device=x.device)
-    io = _product_io(x, ldx, weight, y, x.shape[1], outputs, plan.number_of_types)
-    io.d_plan, io.up, io.rank = plan._words.data_ptr(), up, low.shape[1]
-    io.d_low = low.data_ptr()
-    bias = _set_bias(io, bias)
-    _lib.check(_lib.lib().gn2v_adapted_product(C.byref(io), _stream(x)))
-    return y
 
 
 def _gradient(x, dy, plan, dw, db=None, x_low=False, y_low=False, shared=False):
@@ -290,9 +297,12 @@ def _functions():
             weight_, view = _weights(weight, rows_contiguous=True)
             down_, down_view = _weights(down)
             up_, up_view = _weights(up, rows_contiguous=True)
-            low = _low_rows(rows, ldx, down_view, plan, down.shape[2], scale)
+            rank, low = down.shape[2], None
+            if ctx.needs_input_grad[3]:  # up's gradient is made of the low-rank rows
+                low = torch.empty((x.shape[0], rank), dtype=torch.float32, device=x.device)
             ctx.save_for_backward(x, weight, down, up, low)
-            return _adapted_product(rows, ldx, view, up_view, low, plan, weight.shape[1], bias)
+            return _adapted_product(rows, ldx, view, down_view, up_view, rank, scale, plan,
+                                    weight.shape[1], bias, low)
 
         @staticmethod
         @once_differentiable
@@ -301,16 +311,20 @@ def _functions():
             plan, wanted = ctx.plan, ctx.needs_input_grad
             dx = dw = d_down = d_up = db = None
             dy, ldy = _row_stride(dy)
-            if wanted[0] or wanted[2]:
-                # scale * dy up^T: the rows that both x's and down's gradient are made of
-                up_, up_view = _weights(up)
-                back = _low_rows(dy, ldy, _transposed(up_view), plan, down.shape[2], ctx.scale)
+            rank, back = down.shape[2], None
+            up_, up_view = _weights(up)
             if wanted[0]:
+                # scale * dy up^T, which down's gradient is made of, comes on the way
+                if wanted[2]:
+                    back = torch.empty((x.shape[0], rank), dtype=torch.float32, device=x.device)
                 weight_, view = _weights(weight, rows_contiguous=True)
                 down_, down_view = _weights(down, rows_contiguous=True)
-                dx = _adapted_product(dy, ldy, _transposed(view), _transposed(down_view), back, plan,
-                                      weight.shape[0])
+                dx = _adapted_product(dy, ldy, _transposed(view), _transposed(up_view),
+                                      _transposed(down_view), rank, ctx.scale, plan,
+                                      weight.shape[0], low=back)
             if wanted[2]:
+                if back is None:
+                    back = _low_rows(dy, ldy, _transposed(up_view), plan, rank, ctx.scale)
                 d_down = torch.empty(down.shape, dtype=x.dtype, device=x.device)
                 _gradient(x, back, plan, d_down, y_low=True)
             if wanted[3]:

@@ -340,8 +340,8 @@ int gn2v_touch_rows(float *d_table, uint32_t ld, const uint32_t *d_ids, uint64_t
 /* Rows in the order of their types: a stable counting sort of the type ids (equal types keep the
  * rows' order).  d_types: int32 or int64 ids (type_bytes 4 / 8); an id outside [0, n_types) -- -1,
  * the 0xFFFFFFFF of gn2v_graph_set_types read as int32 -- is an unknown type, and its rows come
- * last.  d_plan int32[plan_words]: order[rows], row_types[rows], offsets[n_types + 2], then the
- * tiles of the product kernels.  d_temp int32[temp_words] is free again once the launch is over.
+ * last.  d_plan int32[plan_words]: order[rows], row_types[rows] (by position), offsets[n_types + 2],
+ * and the types' first tiles (of 64 rows) likewise.  d_temp int32[temp_words] is free again once the launch is over.
  * rows <= 2^31 - 2^20, 1 <= n_types <= GN2V_MAX_TYPES. */
 #define GN2V_MAX_TYPES 32768u
 #define GN2V_MAX_RANK 64u
@@ -376,15 +376,19 @@ typedef struct {
     float scale;
     uint32_t low_rank_rows; /* gn2v_typed_product: y is float32 rows at their POSITIONS in the plan's
                                order (rows of unknown types are left as they were)              */
-    gn2v_weights down;    /* gn2v_few_rows_product, adapted form: K x rank                      */
+    gn2v_weights down;    /* adapted form: K x rank                                             */
     gn2v_weights up;      /* adapted form: rank x N                                             */
-    const float *d_low;   /* gn2v_adapted_product: [rows][rank] as gn2v_typed_product left them */
+    float *d_low;         /* gn2v_adapted_product: [rows][rank], see there                      */
 } gn2v_product_io;
 
 /* y[r] = scale * x[r] W[type of r] + bias[type of r]; rows of unknown types are zeros. */
 int gn2v_typed_product(const gn2v_product_io *io, void *stream);
-/* y[r] = x[r] W + bias + low[position of r] up[type of r]; rows of unknown types: the shared part.
- * low = scale * x[r] down[type of r]: gn2v_typed_product with low_rank_rows. */
+/* y[r] = x[r] W + bias + scale * (x[r] down[type of r]) up[type of r]; rows of unknown types: the
+ * shared part.  d_low is filled with the low-rank rows scale * x[r] down[type of r], at their
+ * positions in the plan's order; it may be NULL where rank <= GN2V_FUSED_RANK and a row holds at
+ * most GN2V_FUSED_ROW_BYTES of inputs: they are then made on the way. */
+#define GN2V_FUSED_RANK 16u
+#define GN2V_FUSED_ROW_BYTES 512u
 int gn2v_adapted_product(const gn2v_product_io *io, void *stream);
 /* Either form for a few rows (rank 0 / > 0), in one launch and without a plan: every row reads the
  * whole weights of its type.  inputs <= GN2V_FEW_ROWS_DEPTH, rows <= 65535, weights with outer = 1. */
