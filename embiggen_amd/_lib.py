@@ -60,6 +60,7 @@ INTERNAL_EXPORTS = [
     # QuantizedTable)
     "gn2v_type_plan_words", "gn2v_type_plan", "gn2v_typed_product", "gn2v_adapted_product",
     "gn2v_few_rows_product", "gn2v_typed_gradient_temp", "gn2v_typed_gradient",
+    "gn2v_adapted_gradient_temp", "gn2v_adapted_gradient",
     "gn2v_table_write", "gn2v_table_read", "gn2v_table_edge_embedding",
 ]
 EXPORTS = BOUNDARY_EXPORTS + INTERNAL_EXPORTS
@@ -277,6 +278,32 @@ class GradientIO(C.Structure):
     ]
 
 
+class AdaptedGradientIO(C.Structure):
+    """gn2v_adapted_gradient_io (include/gn2v_internal.h)."""
+    _fields_ = [
+        ("dtype", C.c_uint32),
+        ("n_types", C.c_uint32),
+        ("rows", C.c_uint64),
+        ("inputs", C.c_uint32),
+        ("outputs", C.c_uint32),
+        ("rank", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("d_x", C.c_void_p),
+        ("d_dy", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("ldy", C.c_int64),
+        ("d_low", C.c_void_p),
+        ("d_back", C.c_void_p),
+        ("d_plan", C.c_void_p),
+        ("d_down", C.c_void_p),
+        ("d_up", C.c_void_p),
+        ("d_dw", C.c_void_p),
+        ("d_db", C.c_void_p),
+        ("d_temp", C.c_void_p),
+        ("temp_bytes", C.c_uint64),
+    ]
+
+
 class Table8(C.Structure):
     """gn2v_table8 (include/gn2v_internal.h)."""
     _fields_ = [("d_codes", C.c_void_p), ("d_scales", C.c_void_p), ("rows", C.c_uint64),
@@ -416,6 +443,8 @@ def lib():
         getattr(L, product).argtypes = [C.POINTER(ProductIO), vp]
     L.gn2v_typed_gradient_temp.argtypes = [C.POINTER(GradientIO), C.POINTER(u64)]
     L.gn2v_typed_gradient.argtypes = [C.POINTER(GradientIO), vp]
+    L.gn2v_adapted_gradient_temp.argtypes = [C.POINTER(AdaptedGradientIO), C.POINTER(u64)]
+    L.gn2v_adapted_gradient.argtypes = [C.POINTER(AdaptedGradientIO), vp]
     L.gn2v_table_write.argtypes = [C.POINTER(Table8), vp, u32, C.c_int64, vp, u32, u64, vp, vp]
     L.gn2v_table_read.argtypes = [C.POINTER(Table8), vp, u32, u64, vp, u32, C.c_int64, vp]
     L.gn2v_table_edge_embedding.argtypes = [C.POINTER(Table8), C.POINTER(Table8), vp, vp, u32, u64,

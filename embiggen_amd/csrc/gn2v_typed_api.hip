@@ -216,22 +216,70 @@ int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, bool narrow, hipS
 // of dw, with no more than 256 MB of partial sums.
 struct GradSizes {
     uint32_t bm, bn, ranges;
-    uint64_t stride, bytes;
+    uint64_t first, second, second_at, stride, bytes;
 };
+
+uint32_t block_of(uint32_t n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+// sums of `first` and `second` elements per range and slot
+void set_sums(GradSizes &g, uint64_t first, uint64_t second, uint64_t tiles, uint64_t ranges) {
+    g.first = first;
+    g.second = second;
+    g.second_at = (first + 3) / 4 * 4;
+    g.stride = (g.second_at + second + 3) / 4 * 4;
+    ranges = std::min<uint64_t>(ranges, (32ull << 20) / g.stride);
+    g.ranges = (uint32_t)std::max<uint64_t>(1, std::min(ranges, tiles));
+    g.bytes = tiles ? 2ull * g.ranges * g.stride * 4 : 0;
+}
 
 GradSizes grad_sizes(const gn2v_gradient_io *io) {
     GradSizes g;
-    g.bm = io->inputs <= 32 ? 32 : io->inputs <= 64 ? 64 : 128;
-    g.bn = io->outputs <= 32 ? 32 : io->outputs <= 64 ? 64 : 128;
+    g.bm = block_of(io->inputs);
+    g.bn = block_of(io->outputs);
     const uint64_t blocks = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm) * ((io->outputs + g.bn - 1) / g.bn);
-    g.stride = (((uint64_t)io->inputs + 1) * io->outputs + 3) / 4 * 4;
-    const uint64_t tiles = tile_bound(io->rows, io->shared ? 0 : io->n_types);
     const uint64_t resident = 256u * gn2v::grad_waves(g.bm / 32, g.bn / 32);
-    uint64_t ranges = std::min<uint64_t>(std::max<uint64_t>(1, resident / blocks), (32ull << 20) / g.stride);
-    ranges = std::max<uint64_t>(1, std::min(ranges, tiles));
-    g.ranges = (uint32_t)ranges;
-    g.bytes = io->rows ? 2 * ranges * g.stride * 4 : 0;
+    set_sums(g, (uint64_t)io->inputs * io->outputs, io->outputs,
+             tile_bound(io->rows, io->shared ? 0 : io->n_types), std::max<uint64_t>(1, resident / blocks));
     return g;
+}
+
+void set_sums(gn2v::GradArgs &a, const GradSizes &g, void *partial, void *dw, void *db) {
+    a.ranges = g.ranges;
+    a.stride = (int64_t)g.stride;
+    a.first = (int64_t)g.first;
+    a.second = (int64_t)g.second;
+    a.second_at = (int64_t)g.second_at;
+    a.partial = (float *)partial;
+    a.dw = dw;
+    a.db = db;
+}
+
+template <typename T>
+void launch_join(const gn2v::GradArgs &a, uint32_t types, hipStream_t s) {
+    // few types lie in many ranges each: sixteen waves share them, four where there are many types
+    const uint64_t blocks = types * (uint64_t)((a.stride + 255) / 256);
+    hipLaunchKernelGGL((gn2v::grad_join_kernel<T>), dim3((unsigned)blocks), dim3(types >= 64 ? 256 : 1024), 0, s, a);
+}
+
+// The adapted form's gradients in one pass over the rows: small enough for one block of sums.  The
+// types' sums and those of the shared weight lie behind one another in d_temp.
+struct FusedSizes {
+    bool fused;
+    GradSizes types, all;
+};
+
+FusedSizes fused_sizes(const gn2v_adapted_gradient_io *io) {
+    FusedSizes f{};
+    f.fused = io->d_down && io->d_up && io->rank <= gn2v::kFusedRank && io->inputs <= 128 && io->outputs <= 128;
+    if (!f.fused) return f;
+    const bool want = io->d_dw || io->d_db;
+    const uint64_t tiles = tile_bound(io->rows, io->n_types + (want ? 1ull : 0ull));
+    f.types.bm = f.all.bm = io->inputs <= 64 ? 64 : 128;
+    f.types.bn = f.all.bn = io->outputs <= 64 ? 64 : 128;
+    set_sums(f.types, (uint64_t)io->inputs * io->rank, (uint64_t)io->rank * io->outputs, tiles,
+             256u * gn2v::adapted_grad_groups((int)size_of(io->dtype)));
+    if (want) set_sums(f.all, io->d_dw ? (uint64_t)io->inputs * io->outputs : 0, io->outputs, tiles, f.types.ranges);
+    return f;
 }
 
 int check_gradient(const gn2v_gradient_io *io) {
@@ -244,6 +292,65 @@ int check_gradient(const gn2v_gradient_io *io) {
     if ((io->x_low && io->inputs > GN2V_MAX_RANK) || (io->y_low && io->outputs > GN2V_MAX_RANK))
         return fail("low-rank rows are at most 64 wide");
     return 0;
+}
+
+int check_adapted_gradient(const gn2v_adapted_gradient_io *io) {
+    if (!io) return fail("NULL io");
+    if (io->dtype != GN2V_F32 && io->dtype != GN2V_BF16) return fail("unknown dtype");
+    if (check_plan(io->rows, io->n_types)) return 1;
+    if (io->inputs == 0 || io->outputs == 0 || io->inputs > (1u << 20) || io->outputs > (1u << 20))
+        return fail("need 1 <= inputs, outputs <= 2^20");
+    if (io->rank == 0 || io->rank > GN2V_MAX_RANK) return fail("need a rank of 1 to 64");
+    return 0;
+}
+
+// the single gradients an adapted form's are made of where they are not fused: 0 down, 1 up, 2 shared
+gn2v_gradient_io part_of(const gn2v_adapted_gradient_io *io, int which) {
+    gn2v_gradient_io g{};
+    g.dtype = io->dtype;
+    g.n_types = io->n_types;
+    g.rows = io->rows;
+    g.inputs = which == 1 ? io->rank : which == 2 && !io->d_dw ? 0 : io->inputs;
+    g.outputs = which == 0 ? io->rank : io->outputs;
+    g.d_x = which == 1 ? (const void *)io->d_low : io->d_x;
+    g.ldx = which == 1 ? (int64_t)io->rank : io->ldx;
+    g.d_dy = which == 0 ? (const void *)io->d_back : io->d_dy;
+    g.ldy = which == 0 ? (int64_t)io->rank : io->ldy;
+    g.x_low = which == 1;
+    g.y_low = which == 0;
+    g.shared = which == 2;
+    g.d_plan = io->d_plan;
+    g.d_dw = which == 0 ? io->d_down : which == 1 ? io->d_up : io->d_dw;
+    g.d_db = which == 2 ? io->d_db : nullptr;
+    g.d_temp = io->d_temp;
+    g.temp_bytes = io->temp_bytes;
+    return g;
+}
+
+bool has_part(const gn2v_adapted_gradient_io *io, int which) {
+    return which == 0 ? io->d_down != nullptr : which == 1 ? io->d_up != nullptr : io->d_dw || io->d_db;
+}
+
+template <typename T, int MI, int NI>
+void launch_fused(const gn2v::AdaptedGradArgs &a, bool want, hipStream_t s) {
+    if (want)
+        hipLaunchKernelGGL((gn2v::adapted_grad_kernel<T, MI, NI, true>), dim3(a.types.ranges), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((gn2v::adapted_grad_kernel<T, MI, NI, false>), dim3(a.types.ranges), dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_fused_grad(const gn2v_adapted_gradient_io *io, const FusedSizes &f, const gn2v::AdaptedGradArgs &a,
+                       hipStream_t s) {
+    const bool want = io->d_dw || io->d_db;
+    if (io->rows) {
+        if (f.types.bm == 64)
+            f.types.bn == 64 ? launch_fused<T, 2, 2>(a, want, s) : launch_fused<T, 2, 4>(a, want, s);
+        else
+            f.types.bn == 64 ? launch_fused<T, 4, 2>(a, want, s) : launch_fused<T, 4, 4>(a, want, s);
+    }
+    launch_join<T>(a.types, io->n_types, s);
+    if (want) launch_join<T>(a.all, 1, s);
 }
 
 template <typename T, int MI, int NI>
@@ -500,8 +607,8 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
     const uint64_t kb = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm), nb = (io->outputs + g.bn - 1) / g.bn;
     const uint64_t blocks = (g.ranges + 7ull) / 8 * 8 * kb * nb;
     const uint32_t types = io->shared ? 1 : io->n_types;
-    const uint64_t joins = types * ((g.stride + 255) / 256);
-    if (blocks > 0x7FFFFFFFull || joins > 0x7FFFFFFFull) return fail("too many blocks for one launch");
+    if (blocks > 0x7FFFFFFFull || types * ((g.stride + 255) / 256) > 0x7FFFFFFFull)
+        return fail("too many blocks for one launch");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_dw ? io->d_dw : io->d_db));
     hipStream_t s = (hipStream_t)stream;
     const uint32_t size = size_of(io->dtype);
@@ -513,15 +620,11 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
     a.x_mode = mode_of(io->d_x, io->ldx, io->inputs, io->x_low ? 4 : size);
     a.y_mode = mode_of(io->d_dy, io->ldy, io->outputs, io->y_low ? 4 : size);
     a.plan = plan_view(io->d_plan, io->rows, io->n_types);
+    a.span = io->shared ? gn2v::kRowBlocks : gn2v::kKnownTiles;
     a.shared = io->shared != 0;
-    a.types = types;
-    a.ranges = g.ranges;
     a.K = (int)io->inputs;
     a.N = (int)io->outputs;
-    a.stride = (int64_t)g.stride;
-    a.partial = (float *)io->d_temp;
-    a.dw = io->d_dw;
-    a.db = io->d_db;
+    set_sums(a, g, io->d_temp, io->d_dw, io->d_db);
     if (io->rows) {
         if (io->dtype == GN2V_F32)
             launch_grad<float>(io, g, a, (unsigned)blocks, s);
@@ -529,12 +632,73 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
             launch_grad<__bf16>(io, g, a, (unsigned)blocks, s);
         HIP_TRY(hipGetLastError());
     }
-    // few types lie in many ranges each: sixteen waves share them, four where there are many types
-    const unsigned threads = types >= 64 ? 256 : 1024;
     if (io->dtype == GN2V_F32)
-        hipLaunchKernelGGL((gn2v::grad_join_kernel<float>), dim3((unsigned)joins), dim3(threads), 0, s, a);
+        launch_join<float>(a, types, s);
     else
-        hipLaunchKernelGGL((gn2v::grad_join_kernel<__bf16>), dim3((unsigned)joins), dim3(threads), 0, s, a);
+        launch_join<__bf16>(a, types, s);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int gn2v_adapted_gradient_temp(const gn2v_adapted_gradient_io *io, uint64_t *temp_bytes) {
+    if (!temp_bytes) return fail("NULL pointer");
+    if (check_adapted_gradient(io)) return 1;
+    const FusedSizes f = fused_sizes(io);
+    *temp_bytes = f.types.bytes + f.all.bytes;
+    if (!f.fused)
+        for (int which = 0; which < 3; ++which)
+            if (has_part(io, which)) {
+                const gn2v_gradient_io g = part_of(io, which);
+                *temp_bytes = std::max<uint64_t>(*temp_bytes, grad_sizes(&g).bytes);
+            }
+    return 0;
+}
+
+int gn2v_adapted_gradient(const gn2v_adapted_gradient_io *io, void *stream) {
+    if (check_adapted_gradient(io)) return 1;
+    if (io->ldx < (int64_t)io->inputs || io->ldy < (int64_t)io->outputs)
+        return fail("row strides must hold a row");
+    if (io->rows && (!io->d_plan || !io->d_x || !io->d_dy || (io->d_down && !io->d_back) || (io->d_up && !io->d_low)))
+        return fail("NULL pointer");
+    uint64_t need = 0;
+    if (gn2v_adapted_gradient_temp(io, &need)) return 1;
+    if (io->temp_bytes < need || (need && !io->d_temp)) return fail("d_temp is too small");
+    const FusedSizes f = fused_sizes(io);
+    if (!f.fused) {
+        for (int which = 0; which < 3; ++which)
+            if (has_part(io, which)) {
+                const gn2v_gradient_io g = part_of(io, which);
+                if (gn2v_typed_gradient(&g, stream)) return 1;
+            }
+        return 0;
+    }
+    DeviceGuard guard(DeviceGuard::of_pointer(io->d_down));
+    const uint32_t size = size_of(io->dtype);
+    const bool want = io->d_dw || io->d_db;
+    gn2v::AdaptedGradArgs a{};
+    gn2v::GradArgs &t = a.types;
+    t.x = io->d_x;
+    t.dy = io->d_dy;
+    t.ldx = io->ldx;
+    t.ldy = io->ldy;
+    t.x_mode = mode_of(io->d_x, io->ldx, io->inputs, size);
+    t.y_mode = mode_of(io->d_dy, io->ldy, io->outputs, size);
+    t.plan = plan_view(io->d_plan, io->rows, io->n_types);
+    t.span = want ? gn2v::kAllTiles : gn2v::kKnownTiles;
+    t.K = (int)io->inputs;
+    t.N = (int)io->outputs;
+    a.all = t;
+    a.all.shared = 1;
+    set_sums(t, f.types, io->d_temp, io->d_down, io->d_up);
+    if (want) set_sums(a.all, f.all, (char *)io->d_temp + f.types.bytes, io->d_dw, io->d_db);
+    a.low = io->d_low;
+    a.back = io->d_back;
+    a.rank = (int)io->rank;
+    a.low_mode = std::max(mode_of(io->d_low, io->rank, io->rank, 4), mode_of(io->d_back, io->rank, io->rank, 4));
+    if (io->dtype == GN2V_F32)
+        launch_fused_grad<float>(io, f, a, (hipStream_t)stream);
+    else
+        launch_fused_grad<__bf16>(io, f, a, (hipStream_t)stream);
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -1053,23 +1053,27 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs a) {
 // second launch joins them in order (no atomics: the same bits in every run).  Either operand may be
 // float32 rows at their positions (the low-rank rows), which enter bfloat16 products as a high and a
 // low part.
+enum GradSpan : int { kKnownTiles = 0, kRowBlocks = 1, kAllTiles = 2 };
+
 struct GradArgs {
     const void *x, *dy;
     int64_t ldx, ldy;
     int x_mode, y_mode;
     PlanView plan;
-    int shared;      // one group: 64 rows after the other, whatever their types
-    uint32_t types;  // of the gradient: 1 if shared
+    int span;        // what is dealt out: the known types' tiles, 64 rows after the other, all tiles
+    int shared;      // one gradient of all of it, not one per type
     uint32_t ranges;
     int K, N;
-    float *partial;  // [range][2][stride]: K * N products, then N column sums
-    int64_t stride;
-    void *dw;        // [type][K][N], may be NULL when only the bias is asked for (K = 0)
-    void *db;        // [type][N] or NULL
+    // sums of a range, float32: [range][2][stride], `first` of them for `dw`, and from second_at (a
+    // multiple of 4) `second` for `db`
+    float *partial;
+    int64_t stride, first, second, second_at;
+    void *dw;        // [type][first]; NULL when only the bias is asked for (K = 0)
+    void *db;        // [type][second] or NULL
 };
-__device__ __forceinline__ int grad_tiles(const GradArgs &a) {  // the known types' tiles
-    return a.shared ? (int)((a.plan.rows + kTileRows - 1) / kTileRows)
-                    : plan_word(a.plan.tile_first, (int)a.plan.types);
+__device__ __forceinline__ int grad_tiles(const GradArgs &a) {
+    return a.span == kRowBlocks ? (int)((a.plan.rows + kTileRows - 1) / kTileRows)
+                                : plan_word(a.plan.tile_first, (int)a.plan.types + (a.span == kAllTiles));
 }
 
 // waves per SIMD that the registers of a block's sums leave room for
@@ -1259,9 +1263,228 @@ __global__ __launch_bounds__(256, grad_waves(MI, NI)) void grad_kernel(GradArgs 
                     if (whole)
                         ((T *)a.db)[(int64_t)now.type * a.N + n] = (T)s;
                     else
-                        part[(int64_t)a.K * a.N + n] = s;
+                        part[a.second_at + n] = s;
                 }
                 sums[ni] = 0.f;
+            }
+        }
+    }
+}
+
+// All gradients of the adapted form at once, for rows and outputs of up to 128 elements and ranks of up
+// to 16: d_down[t] = sum of x[r]^T back[r], d_up[t] = sum of low[r]^T dy[r] over the rows of type t, and
+// (WANT_W) dW = sum of x[r]^T dy[r], db = sum of dy[r] over all rows.  The low-rank rows are further
+// columns of the two LDS tiles, so that x and dy are read once instead of twice.  `types` has the sums
+// per type (dw: d_down, db: d_up), `all` those of the shared weights.
+struct AdaptedGradArgs {
+    GradArgs types, all;
+    const float *low, *back;  // [position][rank]
+    int rank, low_mode;
+};
+
+// workgroups per CU that registers and LDS leave room for
+constexpr int adapted_grad_groups(int size) { return size == 2 ? 3 : 2; }
+
+template <typename T, int MI, int NI, bool WANT_W>
+__global__ __launch_bounds__(256, adapted_grad_groups(sizeof(T))) void adapted_grad_kernel(AdaptedGradArgs a) {
+    constexpr int E = Tile<T>::kChunk, R = 32, STEP = Tile<T>::kSlab;
+    constexpr int BM = 32 * MI, BN = 32 * NI, LOW = sizeof(T) == 4 ? 16 : 32;  // floats, or high | low
+    // row strides as in grad_kernel: lane groups four rows apart fall into different banks
+    constexpr int XW = BM + LOW + (sizeof(T) == 4 ? 4 : 16), YW = BN + LOW + (sizeof(T) == 4 ? 4 : 16);
+    constexpr int XL = R * BM / E / 256, YL = R * BN / E / 256;
+    static_assert(XL >= 1 && YL >= 1, "a block of at least 64 x 64");
+    __shared__ __align__(16) T xss[2][R * XW];
+    __shared__ __align__(16) T yss[2][R * YW];
+    __shared__ int ids[3][kTileRows];
+    const GradArgs &g = a.types;
+    const int tiles = grad_tiles(g);
+    const uint32_t ranges = min(g.ranges, (uint32_t)tiles), range = blockIdx.x;
+    if (range >= ranges) return;
+    const int first = range_first(range, tiles, ranges), last = range_first(range + 1, tiles, ranges);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1, unknown = (int)g.plan.types;
+    f32x4 acc[WANT_W ? MI : 1][WANT_W ? NI : 1] = {}, acc_down[MI / 2] = {}, acc_up[NI / 2] = {};
+    float sums[WANT_W ? NI : 1] = {};
+    u32x4 xr[XL], yr[YL], lr;
+    // half the threads hold four elements of a row of `low`, half of `back`
+    const float *rank_rows = tid < 128 ? a.low : a.back;
+    const int rank_row = (tid & 127) >> 2, rank_at = (tid & 3) * 4;
+    auto fetch = [&](const TileAt &at, const int *id, int r0) {
+        const int count = at.count();
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int c = tid + 256 * i, row = r0 + c / (BM / E);
+            xr[i] = load_chunk((const T *)g.x + (int64_t)id[row] * g.ldx, c % (BM / E) * E, g.K, g.x_mode, row < count);
+        }
+#pragma unroll
+        for (int i = 0; i < YL; ++i) {
+            const int c = tid + 256 * i, row = r0 + c / (BN / E);
+            yr[i] = load_chunk((const T *)g.dy + (int64_t)id[row] * g.ldy, c % (BN / E) * E, g.N, g.y_mode, row < count);
+        }
+        lr = load_chunk(rank_rows + (int64_t)(at.start + r0 + rank_row) * a.rank, rank_at, a.rank, a.low_mode,
+                        r0 + rank_row < count && at.type != unknown);
+    };
+    auto id_at = [&](const TileAt &at) { return tid < at.count() ? g.plan.order[at.start + tid] : 0; };
+    TileAt at = find_tile(g.plan, first, lane), ahead = at, ahead2;
+    if (first + 1 < last) ahead = tile_behind(g.plan, at);
+    ahead2 = ahead;
+    if (first + 2 < last) ahead2 = tile_behind(g.plan, ahead);
+    if (tid < kTileRows) {
+        ids[0][tid] = id_at(at);
+        ids[1][tid] = id_at(ahead);
+    }
+    __syncthreads();
+    fetch(at, ids[0], 0);
+    int slot = 0, buffer = 0;
+    for (int t = first; t < last; ++t) {
+        const TileAt now = at;
+        const int next = slot == 2 ? 0 : slot + 1, free = next == 2 ? 0 : next + 1, count = now.count();
+        for (int r0 = 0; r0 < count; r0 += R) {
+            // a wave that writes this buffer has passed the barrier behind its last readers
+            T *xs = xss[buffer], *ys = yss[buffer];
+            buffer ^= 1;
+#pragma unroll
+            for (int i = 0; i < XL; ++i) {
+                const int c = tid + 256 * i;
+                *reinterpret_cast<u32x4 *>(xs + c / (BM / E) * XW + c % (BM / E) * E) = xr[i];
+            }
+#pragma unroll
+            for (int i = 0; i < YL; ++i) {
+                const int c = tid + 256 * i;
+                *reinterpret_cast<u32x4 *>(ys + c / (BN / E) * YW + c % (BN / E) * E) = yr[i];
+            }
+            T *to = (tid < 128 ? xs + BM + rank_row * XW : ys + BN + rank_row * YW) + rank_at;
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<u32x4 *>(to) = lr;
+            } else {
+                bf16x4 high, rest;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = __uint_as_float(lr[i]);
+                    high[i] = to_bf16(v);
+                    rest[i] = to_bf16(v - (float)high[i]);
+                }
+                *reinterpret_cast<bf16x4 *>(to) = high;
+                *reinterpret_cast<bf16x4 *>(to + 16) = rest;
+            }
+            __syncthreads();
+            const bool ends = r0 + R >= count;
+            int id_ahead = 0;
+            if (ends && t + 2 < last && tid < kTileRows) id_ahead = id_at(ahead2);
+            if (!ends || t + 1 < last) fetch(ends ? ahead : now, ids[ends ? next : slot], ends ? 0 : r0 + R);
+#pragma unroll
+            for (int r = 0; r < R; r += STEP) {
+                if (WANT_W) {
+                    Frag<T> yf[NI];
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) {
+                        yf[ni].columns(ys, YW, (wn * NI + ni) * 16, r, lane);
+                        if (wm == 0 && a.all.db) sums[WANT_W ? ni : 0] += yf[ni].sum();
+                    }
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi) {
+                        Frag<T> xf;
+                        xf.columns(xs, XW, (wm * MI + mi) * 16, r, lane);
+#pragma unroll
+                        for (int ni = 0; ni < NI; ++ni)
+                            acc[WANT_W ? mi : 0][WANT_W ? ni : 0] = mma(yf[ni], xf, acc[WANT_W ? mi : 0][WANT_W ? ni : 0]);
+                    }
+                }
+                if (now.type == unknown) continue;
+                // the waves share the blocks of x's and of dy's columns between them
+                Frag<T> lf;
+                lf.columns(ys, YW, BN, r, lane);
+#pragma unroll
+                for (int i = 0; i < MI / 2; ++i) {
+                    Frag<T> xf;
+                    xf.columns(xs, XW, (wave * MI / 2 + i) * 16, r, lane);
+                    acc_down[i] = mma(lf, xf, acc_down[i]);
+                    if constexpr (sizeof(T) == 2) {
+                        Frag<T> rest;
+                        rest.columns(ys, YW, BN + 16, r, lane);
+                        acc_down[i] = mma(rest, xf, acc_down[i]);
+                    }
+                }
+                lf.columns(xs, XW, BM, r, lane);
+#pragma unroll
+                for (int i = 0; i < NI / 2; ++i) {
+                    Frag<T> yf;
+                    yf.columns(ys, YW, (wave * NI / 2 + i) * 16, r, lane);
+                    acc_up[i] = mma(yf, lf, acc_up[i]);
+                    if constexpr (sizeof(T) == 2) {
+                        Frag<T> rest;
+                        rest.columns(xs, XW, BM + 16, r, lane);
+                        acc_up[i] = mma(yf, rest, acc_up[i]);
+                    }
+                }
+            }
+            if (ends && tid < kTileRows) ids[free][tid] = id_ahead;
+        }
+        slot = next;
+        at = ahead;
+        ahead = ahead2;
+        if (t + 3 < last) ahead2 = tile_behind(g.plan, ahead2);
+        if ((t + 1 < last && at.type == now.type) || now.type == unknown) continue;
+        // the type or the range ends here: the type's sums are whole, or one range's share of them
+        const int type_first = plan_word(g.plan.tile_first, now.type);
+        const int type_last = plan_word(g.plan.tile_first, now.type + 1);
+        const bool whole = type_first >= first && type_last <= last;
+        float *part = g.partial + (int64_t)(2 * range + (type_first >= first)) * g.stride;
+#pragma unroll
+        for (int i = 0; i < MI / 2; ++i) {
+            // lane: rank columns 4 (lane / 16) .. + 3 of row k
+            const int k = (wave * MI / 2 + i) * 16 + (lane & 15), j = 4 * (lane >> 4);
+            const bool vec = (a.rank & 3) == 0;
+            if (k < g.K && whole)
+                store4((T *)g.dw + (int64_t)now.type * g.first + k * a.rank + j, acc_down[i], a.rank - j, vec);
+            else if (k < g.K)
+                store4(part + k * a.rank + j, acc_down[i], a.rank - j, vec);
+            acc_down[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int i = 0; i < NI / 2; ++i) {
+            // lane: columns n .. n + 3 of rank row j
+            const int j = lane & 15, n = (wave * NI / 2 + i) * 16 + 4 * (lane >> 4);
+            const bool vec = (g.N & 3) == 0;
+            if (j < a.rank && whole)
+                store4((T *)g.db + (int64_t)now.type * g.second + j * g.N + n, acc_up[i], g.N - n, vec);
+            else if (j < a.rank)
+                store4(part + g.second_at + j * g.N + n, acc_up[i], g.N - n, vec);
+            acc_up[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    if (WANT_W) {
+        const GradArgs &w = a.all;
+        const bool whole = ranges == 1;
+        float *part = w.partial + (int64_t)(2 * range + (range == 0)) * w.stride;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+            const int k = (wm * MI + mi) * 16 + (lane & 15);
+            if (k >= w.K || !w.dw) continue;
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                const int n = (wn * NI + ni) * 16 + 4 * (lane >> 4);
+                const bool vec = (w.N & 3) == 0;
+                const f32x4 v = acc[WANT_W ? mi : 0][WANT_W ? ni : 0];
+                if (whole)
+                    store4((T *)w.dw + (int64_t)k * w.N + n, v, w.N - n, vec);
+                else
+                    store4(part + (int64_t)k * w.N + n, v, w.N - n, vec);
+            }
+        }
+        if (wm == 0 && w.db) {
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                float s = sums[WANT_W ? ni : 0];
+                s += __shfl_xor(s, 16);
+                s += __shfl_xor(s, 32);
+                const int n = (wn * NI + ni) * 16 + lane;
+                if (lane < 16 && n < w.N) {
+                    if (whole)
+                        ((T *)w.db)[n] = (T)s;
+                    else
+                        part[w.second_at + n] = s;
+                }
             }
         }
     }
@@ -1276,7 +1499,7 @@ __global__ __launch_bounds__(1024) void grad_join_kernel(GradArgs a) {
     const int64_t blocks = (a.stride + 255) / 256;
     const int type = (int)(blockIdx.x / blocks);
     const int64_t at = (int64_t)(blockIdx.x % blocks) * 256 + lane * 4;
-    const int tiles = a.plan.rows ? grad_tiles(a) : 0;
+    const int tiles = a.plan.rows ? grad_tiles(a) : 0;  // no rows: no plan
     const int type_first = a.shared || !tiles ? 0 : a.plan.tile_first[type];
     const int type_last = a.shared || !tiles ? tiles : a.plan.tile_first[type + 1];
     int first = 0, count = 0;  // the ranges it lies in
@@ -1298,14 +1521,13 @@ __global__ __launch_bounds__(1024) void grad_join_kernel(GradArgs a) {
     __syncthreads();
     if (wave == 0) {
         for (int w = 1; w < waves; ++w) sum += part[w][lane];
-        const int64_t weights = (int64_t)a.K * a.N;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t e = at + i;
-            if (e < weights)
-                ((T *)a.dw)[(int64_t)type * weights + e] = (T)sum[i];
-            else if (e < weights + a.N && a.db)
-                ((T *)a.db)[(int64_t)type * a.N + e - weights] = (T)sum[i];
+            const int64_t e = at + i, f = e - a.second_at;
+            if (e < a.first)
+                ((T *)a.dw)[(int64_t)type * a.first + e] = (T)sum[i];
+            else if (f >= 0 && f < a.second && a.db)
+                ((T *)a.db)[(int64_t)type * a.second + f] = (T)sum[i];
         }
     }
 }

@@ -200,21 +200,17 @@ def _low_rows(x, ldx, weight, plan, rank, scale):
     return low
 
 
-def _gradient(x, dy, plan, dw, db=None, x_low=False, y_low=False, shared=False):
-    """Fills dw [types, inputs, outputs] (or [inputs, outputs], ``shared``) and db; ``x`` None: db
-    alone."""
+def _gradient(x, dy, plan, dw, db):
+    """Fills dw [types, inputs, outputs] and db [types, outputs], those that are not None."""
     torch = _torch()
-    dy, ldy = _row_stride(dy)
+    x, ldx = _row_stride(x)
     io = _lib.GradientIO()
-    rows = dy
-    if x is not None:
-        x, io.ldx = _row_stride(x)
-        io.inputs, io.d_x, io.d_dw = x.shape[1], x.data_ptr(), dw.data_ptr()
-        rows = dy if x_low else x
-    io.dtype, io.n_types, io.rows = _dtype(rows), plan.number_of_types, dy.shape[0]
-    io.outputs, io.d_dy, io.ldy = dy.shape[1], dy.data_ptr(), ldy
-    io.x_low, io.y_low, io.shared = x_low, y_low, shared
-    io.d_plan = plan._words.data_ptr()
+    io.dtype, io.n_types, io.rows = _dtype(x), plan.number_of_types, x.shape[0]
+    io.d_x, io.ldx = x.data_ptr(), ldx
+    if dw is not None:
+        io.inputs, io.d_dw = x.shape[1], dw.data_ptr()
+    dy, io.ldy = _row_stride(dy)
+    io.outputs, io.d_dy, io.d_plan = dy.shape[1], dy.data_ptr(), plan._words.data_ptr()
     if db is not None:
         io.d_db = db.data_ptr()
     need = C.c_uint64()
@@ -223,6 +219,28 @@ def _gradient(x, dy, plan, dw, db=None, x_low=False, y_low=False, shared=False):
     temp = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
     io.d_temp, io.temp_bytes = temp.data_ptr(), need.value
     _lib.check(L.gn2v_typed_gradient(C.byref(io), _stream(dy)))
+
+
+def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
+    """Fills the gradients that are not None."""
+    torch = _torch()
+    x, ldx = _row_stride(x)
+    dy, ldy = _row_stride(dy)
+    io = _lib.AdaptedGradientIO()
+    io.dtype, io.n_types, io.rows = _dtype(x), plan.number_of_types, x.shape[0]
+    io.inputs, io.outputs, io.rank = x.shape[1], dy.shape[1], rank
+    io.d_x, io.ldx, io.d_dy, io.ldy = x.data_ptr(), ldx, dy.data_ptr(), ldy
+    io.d_plan = plan._words.data_ptr()
+    for name, tensor in (("d_low", low), ("d_back", back), ("d_down", d_down), ("d_up", d_up),
+                         ("d_dw", dw), ("d_db", db)):
+        if tensor is not None:
+            setattr(io, name, tensor.data_ptr())
+    need = C.c_uint64()
+    L = _lib.lib()
+    _lib.check(L.gn2v_adapted_gradient_temp(C.byref(io), C.byref(need)))
+    temp = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
+    io.d_temp, io.temp_bytes = temp.data_ptr(), need.value
+    _lib.check(L.gn2v_adapted_gradient(C.byref(io), _stream(dy)))
 
 
 # A few rows are worth one launch in which every row reads its type's weights by itself.
@@ -286,7 +304,7 @@ def _functions():
             if ctx.needs_input_grad[1]:
                 dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
             if dw is not None or db is not None:
-                _gradient(x if dw is not None else None, dy, plan, dw, db)
+                _gradient(x, dy, plan, dw, db)
             return dx, dw, db, None
 
     class Adapted(torch.autograd.Function):
@@ -326,16 +344,14 @@ def _functions():
                 if back is None:
                     back = _low_rows(dy, ldy, _transposed(up_view), plan, rank, ctx.scale)
                 d_down = torch.empty(down.shape, dtype=x.dtype, device=x.device)
-                _gradient(x, back, plan, d_down, y_low=True)
             if wanted[3]:
                 d_up = torch.empty(up.shape, dtype=x.dtype, device=x.device)
-                _gradient(low, dy, plan, d_up, x_low=True)
             if wanted[4]:
                 db = torch.empty(weight.shape[1], dtype=x.dtype, device=x.device)
             if wanted[1]:
                 dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
-            if dw is not None or db is not None:
-                _gradient(x if dw is not None else None, dy, plan, dw, db, shared=True)
+            if any(wanted[1:5]):
+                _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db)
             return dx, dw, d_down, d_up, db, None, None
 
     _FUNCTIONS = Typed, Adapted

@@ -416,6 +416,25 @@ typedef struct {
 int gn2v_typed_gradient_temp(const gn2v_gradient_io *io, uint64_t *temp_bytes);
 int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream);
 
+/* All the gradients of the adapted form: d_down[t] = sum over the rows r of type t of x[r]^T back[r],
+ * d_up[t] = sum of low[r]^T dy[r], dw = sum of x[r]^T dy[r] and db = sum of dy[r] over all rows; those
+ * that are NULL are left out.  low and back are float32 rows at their positions as
+ * gn2v_adapted_product leaves them: scale * x down, and scale * dy up^T (the product of dx). */
+typedef struct {
+    uint32_t dtype, n_types;
+    uint64_t rows;
+    uint32_t inputs, outputs, rank, reserved;
+    const void *d_x, *d_dy;
+    int64_t ldx, ldy;
+    const float *d_low, *d_back;
+    const int32_t *d_plan;
+    void *d_down, *d_up, *d_dw, *d_db;
+    void *d_temp;
+    uint64_t temp_bytes;
+} gn2v_adapted_gradient_io;
+int gn2v_adapted_gradient_temp(const gn2v_adapted_gradient_io *io, uint64_t *temp_bytes);
+int gn2v_adapted_gradient(const gn2v_adapted_gradient_io *io, void *stream);
+
 /* Embedding tables in 8 bits: codes u8[rows][stride] and a float32 scale per row and group of
  * `group` (16, 32, 64 or 128) consecutive columns, scales f32[rows][ceil(d / group)]. */
 #define GN2V_INT8 0u
