@@ -410,16 +410,19 @@ gn2v::TableView table_view(const gn2v_table8 *t) {
     return v;
 }
 
-// lanes per row: eight columns each, a power of two, a wave at most
-int lanes_shift(uint32_t d) {
+// lanes per row: `columns` columns each, a power of two, a wave at most
+int lanes_shift(uint32_t d, uint32_t columns) {
     int shift = 0;
-    while (shift < 6 && (8u << shift) < d) ++shift;
+    while (shift < 6 && (columns << shift) < d) ++shift;
     return shift;
 }
 
-unsigned row_blocks(uint64_t n, int shift) {
-    const uint64_t per = 256u >> shift;
-    return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((n + per - 1) / per, 256 * 32));
+// Workgroups of 256 threads for n rows of 1 << shift lanes, `ahead` rows at a time: a step each, but for
+// few rows, which are spread over the CUs (a grid-stride loop over resident workgroups left the last
+// step's waves idle: 333 333 written rows 88 us instead of 62).
+unsigned row_blocks(uint64_t n, int shift, uint64_t ahead) {
+    const uint64_t per = 256u >> shift, all = (n + per - 1) / per;
+    return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(all, 1u << 22), std::max<uint64_t>(512, (all + ahead - 1) / ahead)));
 }
 
 int check_ids(const void *ids, uint32_t id_bytes) {
@@ -430,8 +433,8 @@ int check_ids(const void *ids, uint32_t id_bytes) {
 template <typename T>
 void launch_write(const gn2v_table8 *t, const gn2v::TableView &v, const void *values, int64_t ldv,
                   const void *ids, uint32_t id_bytes, uint64_t n, const int32_t *owner, hipStream_t s) {
-    const int shift = lanes_shift(t->d), mode = mode_of(values, ldv, t->d, sizeof(T));
-    const unsigned blocks = row_blocks(n, shift);
+    const int shift = lanes_shift(t->d, gn2v::kColumns<T>), mode = mode_of(values, ldv, t->d, sizeof(T));
+    const unsigned blocks = row_blocks(n, shift, 2);
     if (t->code == GN2V_INT8)
         hipLaunchKernelGGL((gn2v::table_write_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v,
                            (const T *)values, ldv, mode, ids, (int)id_bytes, n, owner, shift);
@@ -443,8 +446,8 @@ void launch_write(const gn2v_table8 *t, const gn2v::TableView &v, const void *va
 template <typename T>
 void launch_read(const gn2v_table8 *t, const gn2v::TableView &v, const void *ids, uint32_t id_bytes,
                  uint64_t n, void *out, int64_t ldo, hipStream_t s) {
-    const int shift = lanes_shift(t->d), align = alignment(out, ldo, sizeof(T));
-    const unsigned blocks = row_blocks(n, shift);
+    const int shift = lanes_shift(t->d, gn2v::kColumns<T>), align = alignment(out, ldo, sizeof(T));
+    const unsigned blocks = row_blocks(n, shift, gn2v::kAhead);
     if (t->code == GN2V_INT8)
         hipLaunchKernelGGL((gn2v::table_read_kernel<T, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, v, ids,
                            (int)id_bytes, n, (T *)out, ldo, align, shift);
@@ -453,19 +456,20 @@ void launch_read(const gn2v_table8 *t, const gn2v::TableView &v, const void *ids
                            (int)id_bytes, n, (T *)out, ldo, align, shift);
 }
 
-template <uint32_t METHOD>
-void launch_edges(uint32_t code, const gn2v::TableView &a, const gn2v::TableView &b, const void *u,
-                  const void *w, uint32_t id_bytes, uint64_t n, float *out, int64_t ldo, hipStream_t s) {
-    const int shift = lanes_shift(a.d);
-    // Concatenate's second half starts behind the first
-    const int align = std::min(alignment(out, ldo, 4), METHOD == gn2v::kConcatenate ? alignment(out, a.d, 4) : 16);
-    const unsigned blocks = row_blocks(n, shift);
-    if (code == GN2V_INT8)
-        hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kInt8>), dim3(blocks), dim3(256), 0, s, a,
-                           b, u, w, (int)id_bytes, n, out, ldo, align, shift);
-    else
-        hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, gn2v::kE4m3>), dim3(blocks), dim3(256), 0, s, a,
-                           b, u, w, (int)id_bytes, n, out, ldo, align, shift);
+template <uint32_t METHOD, uint32_t CODE>
+void launch_edges(const gn2v::TableView &a, const gn2v::TableView &b, const void *u, const void *w,
+                  uint32_t id_bytes, uint64_t n, float *out, int64_t ldo, hipStream_t s) {
+    if constexpr (METHOD == gn2v::kL2Distance || METHOD == gn2v::kCosineSimilarity) {
+        const int shift = lanes_shift(a.d, 16);
+        hipLaunchKernelGGL((gn2v::table_scores_kernel<METHOD, CODE>), dim3(row_blocks(n, shift, gn2v::kAhead)),
+                           dim3(256), 0, s, a, b, u, w, (int)id_bytes, n, out, ldo, shift);
+    } else {
+        // Concatenate's second half starts behind the first
+        const int shift = lanes_shift(a.d, 4),
+                  align = std::min(alignment(out, ldo, 4), METHOD == gn2v::kConcatenate ? alignment(out, a.d, 4) : 16);
+        hipLaunchKernelGGL((gn2v::table_edges_kernel<METHOD, CODE>), dim3(row_blocks(n, shift, gn2v::kAhead)),
+                           dim3(256), 0, s, a, b, u, w, (int)id_bytes, n, out, ldo, align, shift);
+    }
 }
 
 }  // namespace
@@ -766,7 +770,9 @@ int gn2v_table_edge_embedding(const gn2v_table8 *src, const gn2v_table8 *dst, co
     switch (method) {
 #define GN2V_EDGES(M)                                                                             \
     case gn2v::M:                                                                                 \
-        launch_edges<gn2v::M>(src->code, a, b, d_src_ids, d_dst_ids, id_bytes, n_edges, d_out, ldo, s); \
+        src->code == GN2V_INT8                                                                    \
+            ? launch_edges<gn2v::M, gn2v::kInt8>(a, b, d_src_ids, d_dst_ids, id_bytes, n_edges, d_out, ldo, s) \
+            : launch_edges<gn2v::M, gn2v::kE4m3>(a, b, d_src_ids, d_dst_ids, id_bytes, n_edges, d_out, ldo, s); \
         break
         GN2V_EDGES(kHadamard);
         GN2V_EDGES(kSum);
