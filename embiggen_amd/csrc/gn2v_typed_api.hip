@@ -114,21 +114,22 @@ int check_product(const gn2v_product_io *io) {
     return 0;
 }
 
-// weights of `inputs` x `outputs`
-gn2v::WeightView view_of(const gn2v_weights &w, uint32_t inputs, uint32_t outputs, uint32_t size) {
+// Weights of `inputs` x `outputs` whose inner elements (`wt`) or outer elements are contiguous.  Where
+// an axis has one element its stride says nothing, and both may hold.
+gn2v::WeightView view_of(const gn2v_weights &w, uint32_t inputs, uint32_t outputs, uint32_t size, bool wt) {
     gn2v::WeightView v{w.d_data, w.type_stride, w.inner, w.outer, 0};
-    const int64_t row = w.outer == 1 ? w.inner : w.outer;
-    v.mode = mode_of(w.d_data, row, w.outer == 1 ? outputs : inputs, size, w.type_stride);
+    v.mode = mode_of(w.d_data, wt ? w.outer : w.inner, wt ? inputs : outputs, size, w.type_stride);
     return v;
 }
+bool is_wt(const gn2v_weights &w) { return w.outer != 1; }
 
-gn2v::ProductArgs product_args(const gn2v_product_io *io) {
+gn2v::ProductArgs product_args(const gn2v_product_io *io, bool wt) {
     const uint32_t size = size_of(io->dtype);
     gn2v::ProductArgs a{};
     a.x = io->d_x;
     a.ldx = io->ldx;
     a.x_mode = mode_of(io->d_x, io->ldx, io->inputs, size);
-    a.w = view_of(io->weight, io->inputs, io->outputs, size);
+    a.w = view_of(io->weight, io->inputs, io->outputs, size, wt);
     a.bias = io->d_bias;
     a.bias_type = io->bias_stride;
     a.y = io->d_y;
@@ -194,10 +195,9 @@ void launch_narrow(const gn2v::ProductArgs &a, hipStream_t s) {
 bool is_narrow(uint32_t dtype, uint32_t inputs) { return inputs <= (dtype == GN2V_F32 ? 128u : 256u); }
 
 template <bool ADAPT>
-int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, bool narrow, hipStream_t s) {
+int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, bool wt, bool narrow, hipStream_t s) {
     if ((product_tiles(a, false) + 7) / 8 * 8 * ((a.N + 31) / 32) > 0x7FFFFFFFull)
         return fail("too many tiles for one launch");
-    const bool wt = a.w.outer != 1;
     if (narrow) {
         if (dtype == GN2V_F32)
             wt ? launch_narrow<float, true, ADAPT>(a, s) : launch_narrow<float, false, ADAPT>(a, s);
@@ -506,8 +506,9 @@ int gn2v_typed_product(const gn2v_product_io *io, void *stream) {
     if (io->rows == 0) return 0;
     if (!io->d_plan) return fail("NULL plan");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
-    return launch_product<false>(io->dtype, product_args(io), !io->low_rank_rows && is_narrow(io->dtype, io->inputs),
-                                 (hipStream_t)stream);
+    const bool wt = is_wt(io->weight);
+    return launch_product<false>(io->dtype, product_args(io, wt), wt,
+                                 !io->low_rank_rows && is_narrow(io->dtype, io->inputs), (hipStream_t)stream);
 }
 
 int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
@@ -518,15 +519,21 @@ int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
     if (!io->d_plan || !io->down.d_data || !io->up.d_data) return fail("NULL pointer");
     const bool narrow = io->rank <= gn2v::kFusedRank && is_narrow(io->dtype, io->inputs);
     if (!narrow && !io->d_low) return fail("NULL low-rank rows");
-    if (!narrow && (io->weight.outer == 1) != (io->up.outer == 1) && io->rank > 1)
+    // the kernel of wide rows takes both weights through one path
+    const auto fits = [](const gn2v_weights &w, bool wt, uint32_t inputs, uint32_t outputs) {
+        return wt ? w.inner == 1 || inputs == 1 : w.outer == 1 || outputs == 1;
+    };
+    bool wt = is_wt(io->weight);
+    if (!narrow && !fits(io->up, wt, io->rank, io->outputs)) wt = !wt;
+    if (!narrow && (!fits(io->up, wt, io->rank, io->outputs) || !fits(io->weight, wt, io->inputs, io->outputs)))
         return fail("weight and up must be laid out alike");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_y));
     const uint32_t size = size_of(io->dtype);
-    gn2v::ProductArgs a = product_args(io);
+    gn2v::ProductArgs a = product_args(io, wt);
     a.bias_type = 0;
     a.rank = (int)io->rank;
-    a.down = view_of(io->down, io->inputs, io->rank, size);
-    a.up = view_of(io->up, io->rank, io->outputs, size);
+    a.down = view_of(io->down, io->inputs, io->rank, size, is_wt(io->down));
+    a.up = view_of(io->up, io->rank, io->outputs, size, wt);
     a.low_out = io->d_low;
     hipStream_t s = (hipStream_t)stream;
     if (!narrow) {
@@ -539,11 +546,11 @@ int gn2v_adapted_product(const gn2v_product_io *io, void *stream) {
         low.y_align = alignment(io->d_low, (int64_t)io->rank, 4);
         low.sorted = 1;
         low.N = (int)io->rank;
-        if (launch_product<false>(io->dtype, low, false, s)) return 1;
+        if (launch_product<false>(io->dtype, low, is_wt(io->down), false, s)) return 1;
         a.low = io->d_low;
         a.scale = 1.f;  // the low-rank rows hold it
     }
-    return launch_product<true>(io->dtype, a, narrow, s);
+    return launch_product<true>(io->dtype, a, wt, narrow, s);
 }
 
 int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
@@ -562,7 +569,7 @@ int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
     gn2v::FewArgs a{};
     a.x = io->d_x;
     a.ldx = io->ldx;
-    a.w = view_of(io->weight, io->inputs, io->outputs, size);
+    a.w = view_of(io->weight, io->inputs, io->outputs, size, false);
     a.bias = io->d_bias;
     a.bias_type = io->bias_stride;
     a.y = io->d_y;
@@ -577,8 +584,8 @@ int gn2v_few_rows_product(const gn2v_product_io *io, void *stream) {
     const dim3 grid((io->outputs + 63) / 64, (unsigned)io->rows);
     hipStream_t s = (hipStream_t)stream;
     if (io->rank) {
-        a.down = view_of(io->down, io->inputs, io->rank, size);
-        a.up = view_of(io->up, io->rank, io->outputs, size);
+        a.down = view_of(io->down, io->inputs, io->rank, size, false);
+        a.up = view_of(io->up, io->rank, io->outputs, size, false);
         if (io->dtype == GN2V_F32)
             hipLaunchKernelGGL((gn2v::few_rows_kernel<float, true>), grid, dim3(256), 0, s, a);
         else

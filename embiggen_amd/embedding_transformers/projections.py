@@ -9,15 +9,22 @@ order of the rows by type, and no sorted copy of them is made.  Both can be diff
 are summed in a fixed order, so a run gives the same bits every time.
 """
 import ctypes as C
+import functools
 from typing import Optional, Union
 
 from .. import _lib
 
 
-def _torch():
-    import torch
+_TORCH = None
 
-    return torch
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:  # imported on first use, as everywhere in this package
+        import torch
+
+        _TORCH = torch
+    return _TORCH
 
 
 def _check_rows(name: str, x, dims: int):
@@ -49,7 +56,16 @@ def _check_device(x):
 
 
 def _stream(x):
-    return _torch().cuda.current_stream(x.device).cuda_stream
+    # the raw handle of torch.cuda.current_stream(x.device), a fifth of its time
+    return _torch()._C._cuda_getCurrentRawStream(x.get_device())
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan_words(rows: int, n_types: int):
+    """(words of a plan, words of scratch): a function of the sizes alone."""
+    words, temp_words = C.c_uint64(), C.c_uint64()
+    _lib.check(_lib.lib().gn2v_type_plan_words(rows, n_types, C.byref(words), C.byref(temp_words)))
+    return words.value, temp_words.value
 
 
 class TypePlan:
@@ -76,16 +92,15 @@ class TypePlan:
         self.number_of_types = int(number_of_types)
         self.number_of_rows = types.numel()
         self.device = types.device
-        words, temp_words = C.c_uint64(), C.c_uint64()
-        L = _lib.lib()
-        _lib.check(L.gn2v_type_plan_words(self.number_of_rows, self.number_of_types,
-                                          C.byref(words), C.byref(temp_words)))
+        words, temp_words = _plan_words(self.number_of_rows, self.number_of_types)
         types = types.contiguous()
-        self._words = torch.empty(words.value, dtype=torch.int32, device=types.device)
-        temp = torch.empty(temp_words.value, dtype=torch.int32, device=types.device)
-        _lib.check(L.gn2v_type_plan(types.data_ptr(), types.element_size(), self.number_of_rows,
-                                    self.number_of_types, self._words.data_ptr(), temp.data_ptr(),
-                                    _stream(types)))
+        self._words = torch.empty(words, dtype=torch.int32, device=types.device)
+        temp = None
+        if temp_words:
+            temp = torch.empty(temp_words, dtype=torch.int32, device=types.device)
+        _lib.check(_lib.lib().gn2v_type_plan(
+            types.data_ptr(), types.element_size(), self.number_of_rows, self.number_of_types,
+            self._words.data_ptr(), None if temp is None else temp.data_ptr(), _stream(types)))
 
     @classmethod
     def from_graph(cls, graph, of: str = "nodes", device: int = 0) -> "TypePlan":
@@ -147,30 +162,31 @@ def _dtype(x) -> int:
     return 0 if x.dtype == _torch().float32 else 1
 
 
-def _product_io(x, ldx, weight, y, inputs, outputs, n_types):
-    io = _lib.ProductIO()
-    io.dtype, io.n_types, io.rows = _dtype(x), n_types, x.shape[0]
-    io.inputs, io.outputs, io.scale = inputs, outputs, 1.0
-    io.d_x, io.ldx, io.weight = x.data_ptr(), ldx, weight
-    io.d_y, io.ldy = y.data_ptr(), y.shape[1]
-    return io
+_NO_WEIGHTS = _lib.Weights()
 
 
-def _set_bias(io, bias):
+def _product_io(x, ldx, weight, y, outputs, n_types, bias=None, plan=None, types=None, rank=0,
+                scale=1.0, low_rank_rows=0, down=_NO_WEIGHTS, up=_NO_WEIGHTS, low=None):
+    """(gn2v_product_io, what has to outlive the call)."""
+    bias_stride = 0
     if bias is not None:
         if bias.shape[-1] > 1 and bias.stride(-1) != 1:
             bias = bias.contiguous()
-        io.d_bias = bias.data_ptr()
-        io.bias_stride = bias.stride(0) if bias.dim() == 2 else 0
-    return bias
+        bias_stride = bias.stride(0) if bias.dim() == 2 else 0
+    if types is not None:
+        types = types.contiguous()
+    return _lib.ProductIO(
+        _dtype(x), n_types, x.shape[0], x.shape[1], outputs, x.data_ptr(), ldx, weight,
+        None if bias is None else bias.data_ptr(), bias_stride, y.data_ptr(), y.shape[1],
+        None if plan is None else plan._words.data_ptr(),
+        None if types is None else types.data_ptr(), 0 if types is None else types.element_size(),
+        rank, scale, low_rank_rows, down, up, None if low is None else low.data_ptr()), (bias, types)
 
 
 def _typed_product(x, ldx, weight, plan, outputs, bias=None):
     y = _torch().empty((x.shape[0], outputs), dtype=x.dtype, device=x.device)
-    io = _product_io(x, ldx, weight, y, x.shape[1], outputs, plan.number_of_types)
-    io.d_plan = plan._words.data_ptr()
-    bias = _set_bias(io, bias)
-    _lib.check(_lib.lib().gn2v_typed_product(C.byref(io), _stream(x)))
+    io, keep = _product_io(x, ldx, weight, y, outputs, plan.number_of_types, bias, plan)
+    _lib.check(_lib.lib().gn2v_typed_product(io, _stream(x)))
     return y
 
 
@@ -182,43 +198,54 @@ def _adapted_product(x, ldx, weight, down, up, rank, scale, plan, outputs, bias=
                         or x.shape[1] * x.element_size() > _lib.FUSED_ROW_BYTES):
         low = torch.empty((x.shape[0], rank), dtype=torch.float32, device=x.device)
     y = torch.empty((x.shape[0], outputs), dtype=x.dtype, device=x.device)
-    io = _product_io(x, ldx, weight, y, x.shape[1], outputs, plan.number_of_types)
-    io.d_plan, io.down, io.up, io.rank, io.scale = plan._words.data_ptr(), down, up, rank, scale
-    if low is not None:
-        io.d_low = low.data_ptr()
-    bias = _set_bias(io, bias)
-    _lib.check(_lib.lib().gn2v_adapted_product(C.byref(io), _stream(x)))
+    io, keep = _product_io(x, ldx, weight, y, outputs, plan.number_of_types, bias, plan, None, rank,
+                           scale, 0, down, up, low)
+    _lib.check(_lib.lib().gn2v_adapted_product(io, _stream(x)))
     return y
 
 
 def _low_rows(x, ldx, weight, plan, rank, scale):
     """scale * x[r] W[type of r] as float32 rows at their positions in the plan's order."""
     low = _torch().empty((x.shape[0], rank), dtype=_torch().float32, device=x.device)
-    io = _product_io(x, ldx, weight, low, x.shape[1], rank, plan.number_of_types)
-    io.d_plan, io.scale, io.low_rank_rows = plan._words.data_ptr(), scale, 1
-    _lib.check(_lib.lib().gn2v_typed_product(C.byref(io), _stream(x)))
+    io, keep = _product_io(x, ldx, weight, low, rank, plan.number_of_types, None, plan, None, 0, scale,
+                           1)
+    _lib.check(_lib.lib().gn2v_typed_product(io, _stream(x)))
     return low
+
+
+@functools.lru_cache(maxsize=1024)
+def _gradient_bytes(adapted: bool, *sizes) -> int:
+    """Scratch of a gradient, a function of its sizes and of which parts are wanted: ``sizes`` as the
+    fields of the structure, pointers as truth values."""
+    need = C.c_uint64()
+    L = _lib.lib()
+    if adapted:
+        dtype, n_types, rows, inputs, outputs, rank, down, up, dw, db = sizes
+        io = _lib.AdaptedGradientIO(dtype, n_types, rows, inputs, outputs, rank)
+        io.d_down, io.d_up, io.d_dw, io.d_db = down, up, dw, db
+        _lib.check(L.gn2v_adapted_gradient_temp(io, C.byref(need)))
+    else:
+        io = _lib.GradientIO(*sizes)
+        _lib.check(L.gn2v_typed_gradient_temp(io, C.byref(need)))
+    return need.value
+
+
+def _ptr(tensor):
+    return None if tensor is None else tensor.data_ptr()
 
 
 def _gradient(x, dy, plan, dw, db):
     """Fills dw [types, inputs, outputs] and db [types, outputs], those that are not None."""
     torch = _torch()
     x, ldx = _row_stride(x)
-    io = _lib.GradientIO()
-    io.dtype, io.n_types, io.rows = _dtype(x), plan.number_of_types, x.shape[0]
-    io.d_x, io.ldx = x.data_ptr(), ldx
-    if dw is not None:
-        io.inputs, io.d_dw = x.shape[1], dw.data_ptr()
-    dy, io.ldy = _row_stride(dy)
-    io.outputs, io.d_dy, io.d_plan = dy.shape[1], dy.data_ptr(), plan._words.data_ptr()
-    if db is not None:
-        io.d_db = db.data_ptr()
-    need = C.c_uint64()
-    L = _lib.lib()
-    _lib.check(L.gn2v_typed_gradient_temp(C.byref(io), C.byref(need)))
-    temp = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
-    io.d_temp, io.temp_bytes = temp.data_ptr(), need.value
-    _lib.check(L.gn2v_typed_gradient(C.byref(io), _stream(dy)))
+    dy, ldy = _row_stride(dy)
+    sizes = (_dtype(x), plan.number_of_types, x.shape[0], 0 if dw is None else x.shape[1],
+             dy.shape[1])
+    need = _gradient_bytes(False, *sizes)
+    temp = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    io = _lib.GradientIO(*sizes, x.data_ptr(), dy.data_ptr(), ldx, ldy, 0, 0, 0, 0,
+                         plan._words.data_ptr(), _ptr(dw), _ptr(db), temp.data_ptr(), need)
+    _lib.check(_lib.lib().gn2v_typed_gradient(io, _stream(dy)))
 
 
 def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
@@ -226,21 +253,14 @@ def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
     torch = _torch()
     x, ldx = _row_stride(x)
     dy, ldy = _row_stride(dy)
-    io = _lib.AdaptedGradientIO()
-    io.dtype, io.n_types, io.rows = _dtype(x), plan.number_of_types, x.shape[0]
-    io.inputs, io.outputs, io.rank = x.shape[1], dy.shape[1], rank
-    io.d_x, io.ldx, io.d_dy, io.ldy = x.data_ptr(), ldx, dy.data_ptr(), ldy
-    io.d_plan = plan._words.data_ptr()
-    for name, tensor in (("d_low", low), ("d_back", back), ("d_down", d_down), ("d_up", d_up),
-                         ("d_dw", dw), ("d_db", db)):
-        if tensor is not None:
-            setattr(io, name, tensor.data_ptr())
-    need = C.c_uint64()
-    L = _lib.lib()
-    _lib.check(L.gn2v_adapted_gradient_temp(C.byref(io), C.byref(need)))
-    temp = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
-    io.d_temp, io.temp_bytes = temp.data_ptr(), need.value
-    _lib.check(L.gn2v_adapted_gradient(C.byref(io), _stream(dy)))
+    sizes = (_dtype(x), plan.number_of_types, x.shape[0], x.shape[1], dy.shape[1], rank)
+    parts = (d_down, d_up, dw, db)
+    need = _gradient_bytes(True, *sizes, *(t is not None for t in parts))
+    temp = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    io = _lib.AdaptedGradientIO(*sizes, 0, x.data_ptr(), dy.data_ptr(), ldx, ldy, _ptr(low),
+                                _ptr(back), plan._words.data_ptr(), *(_ptr(t) for t in parts),
+                                temp.data_ptr(), need)
+    _lib.check(_lib.lib().gn2v_adapted_gradient(io, _stream(dy)))
 
 
 # A few rows are worth one launch in which every row reads its type's weights by itself.
@@ -256,19 +276,17 @@ def _few_rows(x, plan, types, weight, number_of_types, bias=None, down=None, up=
     if any(w is not None and w.shape[-1] > 1 and w.stride(-1) != 1 for w in (weight, down, up)):
         return None  # transposed weights would be copied whole
     x, ldx = _row_stride(x)
-    weight, view = _weights(weight, rows_contiguous=True)
+    weight, view = _weights(weight, True)
     y = _torch().empty((rows, outputs), dtype=x.dtype, device=x.device)
-    io = _product_io(x, ldx, view, y, inputs, outputs, number_of_types)
     if plan is not None:
-        io.d_plan = plan._words.data_ptr()
+        types = None
+    if down is None:
+        io, keep = _product_io(x, ldx, view, y, outputs, number_of_types, bias, plan, types)
     else:
-        types = types.contiguous()
-        io.d_types, io.type_bytes = types.data_ptr(), types.element_size()
-    bias = _set_bias(io, bias)
-    if down is not None:
-        (down, io.down), (up, io.up) = _weights(down, True), _weights(up, True)
-        io.rank, io.scale = down.shape[2], scale
-    _lib.check(_lib.lib().gn2v_few_rows_product(C.byref(io), _stream(x)))
+        (down, down_view), (up, up_view) = _weights(down, True), _weights(up, True)
+        io, keep = _product_io(x, ldx, view, y, outputs, number_of_types, bias, plan, types,
+                               down.shape[2], scale, 0, down_view, up_view)
+    _lib.check(_lib.lib().gn2v_few_rows_product(io, _stream(x)))
     return y
 
 
@@ -280,6 +298,12 @@ def _functions():
     torch = _torch()
     from torch.autograd.function import once_differentiable
 
+    def once(backward):
+        # the check for a second differentiation costs more than a launch: made where gradients of
+        # gradients are recorded at all
+        checked = once_differentiable(backward)
+        return staticmethod(lambda ctx, dy: (checked if torch.is_grad_enabled() else backward)(ctx, dy))
+
     class Typed(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, weight, bias, plan):
@@ -289,8 +313,7 @@ def _functions():
             weight, view = _weights(weight)
             return _typed_product(x, ldx, view, plan, weight.shape[2], bias)
 
-        @staticmethod
-        @once_differentiable
+        @once
         def backward(ctx, dy):
             x, weight = ctx.saved_tensors
             plan = ctx.plan
@@ -322,8 +345,7 @@ def _functions():
             return _adapted_product(rows, ldx, view, down_view, up_view, rank, scale, plan,
                                     weight.shape[1], bias, low)
 
-        @staticmethod
-        @once_differentiable
+        @once
         def backward(ctx, dy):
             x, weight, down, up, low = ctx.saved_tensors
             plan, wanted = ctx.plan, ctx.needs_input_grad

@@ -7,23 +7,20 @@ per row and group of columns -- 0.26 to 0.31 of the bytes at 128 columns --, qua
 written and gives them back as float32 or bfloat16; ``edge_embedding`` and ``EdgeTransformer`` read the
 8-bit rows directly.
 """
-import ctypes as C
 from typing import Optional
 
 from .. import _lib
+from .projections import _stream, _torch
 
 GROUP_SIZES = (16, 32, 64, 128)
-
-
-def _torch():
-    import torch
-
-    return torch
+_CODES = {}
 
 
 def _codes():
-    torch = _torch()
-    return {torch.int8: 0, torch.float8_e4m3fn: 1}
+    if not _CODES:
+        torch = _torch()
+        _CODES.update({torch.int8: 0, torch.float8_e4m3fn: 1})
+    return _CODES
 
 
 def _ids(rows, device, what: str):
@@ -93,7 +90,7 @@ class QuantizedTable:
                              f"but it is on {codes.device}.")
         if codes.data_ptr() % 16:
             raise ValueError("The codes should be aligned to 16 bytes.")
-        self.codes, self.scales = codes, scales
+        self._codes, self._scales = codes, scales
         self.embedding_size, self.group_size = size, group_size
         self._io = _lib.Table8(codes.data_ptr(), scales.data_ptr(), codes.shape[0], size,
                                codes.shape[1], group_size, _codes()[codes.dtype])
@@ -140,6 +137,16 @@ class QuantizedTable:
         return new
 
     @property
+    def codes(self):
+        """int8 or float8_e4m3fn [rows, stride]: the tensor itself, not a copy."""
+        return self._codes
+
+    @property
+    def scales(self):
+        """float32 [rows, groups]: the tensor itself, not a copy."""
+        return self._scales
+
+    @property
     def shape(self):
         return (self.codes.shape[0], self.embedding_size)
 
@@ -149,9 +156,6 @@ class QuantizedTable:
 
     def __len__(self) -> int:
         return self.codes.shape[0]
-
-    def _stream(self):
-        return _torch().cuda.current_stream(self.device).cuda_stream
 
     def write(self, values, rows=None):
         """Quantises ``values`` [entries, embedding_size] (float32 or bfloat16; rows may be strided)
@@ -181,9 +185,9 @@ class QuantizedTable:
         if rows is not None and n > _lib.TABLE_FEW_ENTRIES:
             owner = torch.empty(len(self), dtype=torch.int32, device=self.device)
         _lib.check(_lib.lib().gn2v_table_write(
-            C.byref(self._io), values.data_ptr(), kind, max(values.stride(0), values.shape[1]),
+            self._io, values.data_ptr(), kind, max(values.stride(0), values.shape[1]),
             None if rows is None else rows.data_ptr(), 0 if rows is None else rows.element_size(), n,
-            None if owner is None else owner.data_ptr(), self._stream()))
+            None if owner is None else owner.data_ptr(), _stream(self.codes)))
 
     def read(self, rows=None, dtype=None):
         """The rows ``rows`` (int32 / int64; by default all) as a float32 (or bfloat16: ``dtype``)
@@ -196,9 +200,9 @@ class QuantizedTable:
         n = len(self) if rows is None else rows.numel()
         out = torch.empty((n, self.embedding_size), dtype=dtype, device=self.device)
         _lib.check(_lib.lib().gn2v_table_read(
-            C.byref(self._io), None if rows is None else rows.data_ptr(),
+            self._io, None if rows is None else rows.data_ptr(),
             0 if rows is None else rows.element_size(), n, out.data_ptr(), kind,
-            self.embedding_size, self._stream()))
+            self.embedding_size, _stream(self.codes)))
         return out
 
 
@@ -221,6 +225,6 @@ def quantized_edge_embedding(table, sources, destinations, method: int, width: i
         src, dst = src.long(), dst.long()
     out = torch.empty((src.numel(), width), dtype=torch.float32, device=table.device)
     _lib.check(_lib.lib().gn2v_table_edge_embedding(
-        C.byref(table._io), C.byref(other._io), src.data_ptr(), dst.data_ptr(), src.element_size(),
-        src.numel(), method, out.data_ptr(), width, table._stream()))
+        table._io, other._io, src.data_ptr(), dst.data_ptr(), src.element_size(),
+        src.numel(), method, out.data_ptr(), width, _stream(table.codes)))
     return out

@@ -234,7 +234,8 @@ def test_plan_of_ids_beyond_32_bits_and_of_a_graph():
 SHAPES = [  # rows, types, inputs, outputs
     (1, 1, 1, 1), (1, 3, 128, 128), (7, 2, 3, 5), (48, 7, 100, 100), (64, 1, 32, 32),
     (65, 3, 33, 31), (129, 5, 64, 65), (200, 300, 17, 129), (1025, 4, 100, 71),
-    (3001, 9, 130, 96), (5000, 3, 256, 200), (2049, 1, 128, 128),
+    (3001, 9, 130, 96), (5000, 3, 256, 200), (2049, 1, 128, 128), (300, 4, 300, 1), (300, 4, 1, 300),
+    (700, 3, 513, 140), (90, 2, 5000, 10),
 ]
 
 
@@ -361,7 +362,9 @@ ADAPTED = [  # rows, types, inputs, outputs, rank, skew
     (1, 1, 1, 1, 1, False), (1, 4, 64, 64, 8, False), (33, 64, 128, 96, 16, False),
     (50, 3, 100, 100, 5, False), (64, 2, 33, 40, 33, False), (130, 200, 40, 70, 16, False),
     (700, 3, 100, 130, 64, True), (1500, 1, 65, 33, 7, False), (4000, 37, 128, 128, 16, True),
-    (2100, 900, 50, 64, 4, False), (3000, 6, 200, 32, 32, True),
+    (2100, 900, 50, 64, 4, False), (3000, 6, 200, 32, 32, True), (300, 4, 40, 1, 20, False),
+    (300, 4, 1, 40, 20, False), (150, 3, 1, 1, 1, False), (400, 3, 300, 1, 1, False),
+    (400, 3, 1, 300, 1, False), (500, 4, 300, 260, 16, False), (260, 5, 140, 130, 9, True),
 ]
 
 
