@@ -218,7 +218,7 @@ MAX_RANK = 64                # GN2V_MAX_RANK
 FUSED_RANK = 16              # GN2V_FUSED_RANK
 FUSED_ROW_BYTES = 512        # GN2V_FUSED_ROW_BYTES
 FEW_ROWS_DEPTH = 4096        # GN2V_FEW_ROWS_DEPTH
-TABLE_FEW_ENTRIES = 1024     # GN2V_TABLE_FEW_ENTRIES
+TABLE_FEW_ENTRIES = 512      # GN2V_TABLE_FEW_ENTRIES
 
 
 class Weights(C.Structure):

@@ -20,7 +20,7 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 64;     // rows of a product tile
 constexpr int kMaxTypes = 32768;  // the plan counts the types in LDS: 128 KB
-constexpr int kSmallPlan = 1024;  // rows one workgroup sorts in LDS
+constexpr int kSmallPlan = 512;   // rows one workgroup sorts in LDS
 
 // ------------------------------------------------------------------------------------ the plan
 // int32 words: order[rows] (row id at every position), row_types[rows] (type at every position;
@@ -38,7 +38,8 @@ __device__ __forceinline__ int type_at(const I *types, uint32_t row, uint32_t n_
     return t >= 0 && (uint64_t)t < (uint64_t)n_types ? (int)t : (int)n_types;
 }
 
-// Up to 1 024 rows: one workgroup sorts (type << 10 | row) in LDS -- one launch.
+// Up to 512 rows: one workgroup sorts (type << 10 | row) in LDS -- one launch, bound by the sort's
+// barriers (64 rows 6 us, 512 rows 10 us: as long as the three launches below).
 template <typename I>
 __global__ __launch_bounds__(kSmallPlan) void plan_small_kernel(const I *__restrict__ types, PlanView p) {
     __shared__ uint32_t key[kSmallPlan];
@@ -97,7 +98,8 @@ __global__ __launch_bounds__(kSmallPlan) void plan_small_kernel(const I *__restr
 // More rows: a workgroup per stripe of rows counts its types in LDS; the counts of the stripes before
 // it and of the smaller types say where its rows go.  Equal types keep their rows' order (a wave
 // takes a part of the stripe in order and ranks 64 rows at a time by ballots over the bits of their
-// types), so sums over a type's rows have the same order in every run.
+// types), so sums over a type's rows have the same order in every run.  Three launches of latency: 169 343
+// rows of 40 types 12 us, 1 M rows of 20 types 19 us (its 8 bytes read and 8 written a row: 3 us).
 template <typename I>
 __global__ __launch_bounds__(256) void plan_count_kernel(const I *__restrict__ types, uint32_t rows,
                                                          uint32_t n_types, uint32_t stripe,
@@ -140,24 +142,25 @@ __global__ __launch_bounds__(256) void plan_scan_kernel(int *__restrict__ counts
     if (lane == 0) totals[t] = carry;
 }
 
-// LDS: next[waves][n_types + 1].
+// LDS: next[parts][n_types + 1].  The first `parts` waves place rows, all of them sum over the types.
 template <typename I>
-__global__ __launch_bounds__(256) void plan_place_kernel(const I *__restrict__ types, PlanView p,
-                                                         uint32_t stripe, uint32_t stripes,
-                                                         const int *__restrict__ counts, int bits,
-                                                         const int *__restrict__ totals) {
+__global__ __launch_bounds__(1024) void plan_place_kernel(const I *__restrict__ types, PlanView p,
+                                                          uint32_t stripe, uint32_t stripes,
+                                                          const int *__restrict__ counts, int bits,
+                                                          const int *__restrict__ totals, uint32_t parts) {
     extern __shared__ int next[];
-    __shared__ int sums[2][4];
+    __shared__ int sums[2][16];
     const uint32_t groups = p.types + 1, threads = blockDim.x, waves = threads >> 6;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t t = threadIdx.x; t < groups * waves; t += threads) next[t] = 0;
+    for (uint32_t t = threadIdx.x; t < groups * parts; t += threads) next[t] = 0;
     __syncthreads();
-    // the rows of the waves' own parts of the stripe
+    // the rows of the wave's own part of the stripe
     const uint64_t first = (uint64_t)blockIdx.x * stripe;
     const uint64_t last = first + stripe < p.rows ? first + stripe : p.rows;
-    const uint32_t part = ((stripe + waves - 1) / waves + 63) / 64 * 64;
-    const uint64_t from = min(first + (uint64_t)wave * part, last), to = min(from + part, last);
-    if (waves > 1)
+    const uint32_t part = ((stripe + parts - 1) / parts + 63) / 64 * 64;
+    const uint64_t from = wave < (int)parts ? min(first + (uint64_t)wave * part, last) : last;
+    const uint64_t to = min(from + part, last);
+    if (parts > 1)
         for (uint64_t r = from + lane; r < to; r += 64)
             atomicAdd(&next[wave * groups + type_at(types, (uint32_t)r, p.types)], 1);
     __syncthreads();
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(256) void plan_place_kernel(const I *__restrict__ t
                 p.tile_first[t] = start_tiles;
             }
             int at = start + before;
-            for (uint32_t w = 0; w < waves; ++w) {
+            for (uint32_t w = 0; w < parts; ++w) {
                 const int own = next[w * groups + t];
                 next[w * groups + t] = at;
                 at += own;
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(256) void plan_place_kernel(const I *__restrict__ t
         p.offsets[groups] = carry;
         p.tile_first[groups] = carry_tiles;
     }
-    // every wave walks its own part: its counters belong to no other wave
+    // every such wave walks its own part: its counters belong to no other wave
     volatile int *mine = next + wave * groups;
     for (uint64_t base = from; base < to; base += 256) {
         int type4[4];
@@ -336,6 +339,16 @@ __device__ __forceinline__ u32x4 load_chunk(const T *row, int k, int length, int
 
 // nearest bfloat16 (ties to even; NaN stays NaN)
 __device__ __forceinline__ __bf16 to_bf16(float v) { return (__bf16)v; }
+
+// A float as two bfloat16 parts, 2^-16 of it left out at most: its upper half, and what that leaves,
+// rounded to nearest.  Both have its sign and neither is zero unless it is: an infinite factor makes the
+// same infinity of both parts, not a NaN.
+__device__ __forceinline__ void split(float v, __bf16 &high, __bf16 &rest) {
+    const uint32_t bits = __float_as_uint(v) & 0xFFFF0000u;
+    high = __builtin_bit_cast(__bf16, (uint16_t)(bits >> 16));
+    const float left = v - __uint_as_float(bits);  // exact; NaN of an infinity
+    rest = to_bf16(__builtin_fabsf(left) > 0.f ? left : __builtin_copysignf(v != 0.f ? 0x1p-126f : 0.f, v));
+}
 
 // four consecutive output elements, `valid` of them inside the row
 __device__ __forceinline__ void store4(float *p, f32x4 v, int valid, bool vec) {
@@ -469,7 +482,7 @@ struct ProductArgs {
     void *y;           // rows at their ids; `sorted`: float32 rows at their positions
     int64_t ldy;
     int y_align, sorted;
-    float scale;       // of the product (before the bias)
+    float scale;       // of the product (before the bias); narrow_product_kernel, adapted form: of x down
     PlanView plan;
     int K, N;
     // adapted form: low[position][rank] float32 times the `up` weights of the row's type
@@ -607,10 +620,15 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
             const int own = types[lane];
             const bool begins = own < (int)a.plan.types && (lane == 0 || types[lane - 1] != own);
             unsigned long long runs = __ballot(begins);
-            if (__popcll(runs) <= 4) {
-                // Few runs: 32 rank columns at a time, rows of other types zero.  In bfloat16 the
-                // low-rank rows enter as a high and a low part, 16 bits of them together.
+            // Measured on 32 768 rows of 512 -> 256 (rank 16) and 1 024 -> 1 024 (rank 32), float32 and
+            // bfloat16: 16 runs a tile 381 / 1 593 / 169 / 628 us this way, 423 / 1 584 / 205 / 867 the other;
+            // 64 runs 1 183 / 4 160 / 571 / 1 877 and 1 079 / 2 567 / 510 / 1 137.
+            if (__popcll(runs) <= 16) {
+                // Few runs: 32 rank columns at a time.  Every run is a product of the whole tile in sums of
+                // its own, which only its rows take: weights that are infinite or NaN reach no row of
+                // another type.  In bfloat16 the low-rank rows enter as a high and a low part.
                 for (; runs; runs &= runs - 1) {
+                    f32x4 run[MI][NI] = {};
                     const int t = types[__ffsll(runs) - 1];
                     const T *up = (const T *)a.up.data + (int64_t)t * a.up.type;
                     for (int j0 = 0; j0 < a.rank; j0 += 32) {
@@ -623,9 +641,10 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
                             if constexpr (sizeof(T) == 4) {
                                 xs[row * XS + (i & 31)] = v;
                             } else {
-                                const __bf16 high = to_bf16(v);
+                                __bf16 high, rest;
+                                split(v, high, rest);
                                 xs[row * XS + (i & 31)] = high;
-                                xs[row * XS + 32 + (i & 31)] = to_bf16(v - (float)high);
+                                xs[row * XS + 32 + (i & 31)] = rest;
                             }
                         }
                         put_w();
@@ -643,10 +662,16 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
                             for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
                                 for (int ni = 0; ni < NI; ++ni)
-                                    acc[mi][ni] = mma(wf[ni], xf[mi], acc[mi][ni]);
+                                    run[mi][ni] = mma(wf[ni], xf[mi], run[mi][ni]);
                         }
                         __syncthreads();
                     }
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+                        if (types[m0 + mi * 16 + (lane & 15)] == t) {
+#pragma unroll
+                            for (int ni = 0; ni < NI; ++ni) acc[mi][ni] += run[mi][ni];
+                        }
                 }
             } else {
                 // Many types, few rows each: every lane adds its row's part from its row's weights.
@@ -900,7 +925,9 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
                             low = mma(af, xf, low);
                         }
                         const int row = wave * 16 + (lane & 15), j = 4 * (lane >> 4);
-                        low *= a.scale;
+                        // columns behind the rank stay zero, also where the row holds an infinity
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) low[i] = j + i < a.rank ? low[i] * a.scale : 0.f;
                         if (a.low_out && column == 0 && r0 + row < count)
                             store4(a.low_out + (int64_t)(start + r0 + row) * a.rank + j, low, a.rank - j,
                                    (a.rank & 3) == 0);
@@ -910,8 +937,10 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
                             bf16x4 high, rest;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                high[i] = to_bf16(low[i]);
-                                rest[i] = to_bf16(low[i] - (float)high[i]);
+                                __bf16 h, r;
+                                split(low[i], h, r);
+                                high[i] = h;
+                                rest[i] = r;
                             }
                             *reinterpret_cast<bf16x4 *>(ls + row * LS + j) = high;
                             *reinterpret_cast<bf16x4 *>(ls + row * LS + 16 + j) = rest;
@@ -939,7 +968,9 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
                 float v[4 * NI];
 #pragma unroll
                 for (int i = 0; i < 4 * NI; ++i)
-                    v[i] = ADAPT || known ? acc[mi][i % NI][i / NI] + bias[i] : 0.f;
+                    v[i] = ADAPT   ? acc[mi][i % NI][i / NI] + bias[i]
+                           : known ? acc[mi][i % NI][i / NI] * a.scale + bias[i]
+                                   : 0.f;
                 if constexpr (NI == 2)
                     store8(y, v, a.N - n, a.y_align);
                 else
@@ -1040,6 +1071,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs a) {
     if (tid < 64 && n0 + tid < a.N) {
         float s = 0.f;
         for (int i = 0; i < SPLIT; ++i) s += part[i * 64 + tid];
+        if (!ADAPT) s *= a.scale;
         if (a.bias) s += (float)((const T *)a.bias)[(ADAPT ? 0 : (int64_t)type * a.bias_type) + n0 + tid];
         y[n0 + tid] = (T)s;
     }
@@ -1114,9 +1146,10 @@ __global__ __launch_bounds__(256, grad_waves(MI, NI)) void grad_kernel(GradArgs 
         bf16x8 h, l;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float v = __uint_as_float(i < 4 ? q0[i & 3] : q1[i & 3]);
-            h[i] = to_bf16(v);
-            l[i] = to_bf16(v - (float)h[i]);
+            __bf16 upper, rest;
+            split(__uint_as_float(i < 4 ? q0[i & 3] : q1[i & 3]), upper, rest);
+            h[i] = upper;
+            l[i] = rest;
         }
         high = __builtin_bit_cast(u32x4, h);
         low = __builtin_bit_cast(u32x4, l);
@@ -1360,9 +1393,10 @@ __global__ __launch_bounds__(256, adapted_grad_groups(sizeof(T))) void adapted_g
                 bf16x4 high, rest;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float v = __uint_as_float(lr[i]);
-                    high[i] = to_bf16(v);
-                    rest[i] = to_bf16(v - (float)high[i]);
+                    __bf16 h, r;
+                    split(__uint_as_float(lr[i]), h, r);
+                    high[i] = h;
+                    rest[i] = r;
                 }
                 *reinterpret_cast<bf16x4 *>(to) = high;
                 *reinterpret_cast<bf16x4 *>(to + 16) = rest;

@@ -263,15 +263,21 @@ def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
     _lib.check(_lib.lib().gn2v_adapted_gradient(io, _stream(dy)))
 
 
-# A few rows are worth one launch in which every row reads its type's weights by itself.
-FEW_ROWS = 64
+# A few rows are worth one launch in which every row reads its type's weights by itself: while there are
+# at most so many, and what they read together is at most so many bytes.  One launch / plan and product
+# (the plan given), microseconds: 128 -> 128 float32, 1 024 rows 6.4 / 20.5 (10.2), 4 096 rows 16.6 / 22.4
+# (11.7); 512 -> 256, 512 rows (268 MB) float32 15.7 / 44.4 (34.9), 1 024 rows bfloat16 (268 MB) 18.3 /
+# 23.6 (13.6), 2 048 rows (537 MB) 32.4 / 23.2 (13.7); 1 024 -> 1 024, 64 rows (268 MB) float32 18.1 / 68.4.
+FEW_ROWS = 1024
+FEW_BYTES = 1 << 28
 
 
 def _few_rows(x, plan, types, weight, number_of_types, bias=None, down=None, up=None, scale=1.0):
     """The one-launch form, or None where it does not apply."""
     rows, inputs = x.shape
     outputs = weight.shape[-1]
-    if not 0 < rows <= FEW_ROWS or inputs > _lib.FEW_ROWS_DEPTH:
+    if (not 0 < rows <= FEW_ROWS or inputs > _lib.FEW_ROWS_DEPTH
+            or rows * inputs * outputs * x.element_size() > FEW_BYTES):
         return None
     if any(w is not None and w.shape[-1] > 1 and w.stride(-1) != 1 for w in (weight, down, up)):
         return None  # transposed weights would be copied whole

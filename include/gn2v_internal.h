@@ -454,7 +454,7 @@ typedef struct {
  * ties to even; a group with an infinity or a NaN reads back as NaN.  Entries whose id lies outside
  * the table are left out; of several entries of one row the last is kept.  d_owner int32[rows]:
  * scratch, needed with ids and n > GN2V_TABLE_FEW_ENTRIES.  n < 2^31. */
-#define GN2V_TABLE_FEW_ENTRIES 1024u
+#define GN2V_TABLE_FEW_ENTRIES 512u
 int gn2v_table_write(const gn2v_table8 *table, const void *d_values, uint32_t dtype, int64_t ldv,
                      const void *d_ids, uint32_t id_bytes, uint64_t n, int32_t *d_owner, void *stream);
 /* out[i] = row ids[i] (NULL: row i), zeros where the id lies outside the table. */

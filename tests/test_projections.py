@@ -194,9 +194,12 @@ def test_weight_views_need_no_copies():
 
 # ------------------------------------------------------------------------------------ the plan
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,types", [(0, 3), (1, 1), (1, 7), (63, 2), (64, 1), (65, 5), (1000, 3),
+@pytest.mark.parametrize("rows,types", [(0, 3), (1, 1), (1, 7), (63, 2), (64, 1), (65, 5), (511, 3), (512, 300),
+                                        (513, 300), (1000, 3),
                                         (1024, 4000), (1025, 5), (5000, 1), (70_001, 37),
-                                        (20_000, 20_000), (3000, 32_768)])
+                                        (20_000, 20_000), (3000, 32_768),
+                                        # counters that end at 64 KB of LDS, and just behind
+                                        (5000, 4094), (5000, 4095), (5000, 4096), (2000, 16_383)])
 @pytest.mark.parametrize("id_type", [torch.int32, torch.int64])
 def test_plan_is_the_stable_order(rows, types, id_type):
     gen = torch.Generator().manual_seed(rows + types)
@@ -422,6 +425,59 @@ def test_rows_without_an_adapter_get_the_shared_part(rows, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("inputs,rank", [(40, 5), (40, 20), (300, 5)])
+def test_a_types_infinities_reach_no_other_type(rows, inputs, rank, dtype):
+    """Adapters that hold infinities or NaN, forward and backward: rows, and gradients, of the other
+    types are what they are without them."""
+    ids, (x, w, down, up, b, dy) = make(rows, 3, (rows, inputs), (inputs, 70), (3, inputs, rank),
+                                        (3, rank, 70), (70,), (rows, 70), dtype=dtype)
+    want, tolerance = adapted_reference(x, w, down, up, ids, b, 1.0, dy, dtype)
+    for value, place in ((float("inf"), up), (float("nan"), down)):
+        kept = place[1].clone()
+        place[1] = value
+        leaves = [v.cuda().requires_grad_() for v in (x, down, up)]
+        y = E.adapted_projection(leaves[0], w.cuda(), leaves[1], leaves[2], ids.cuda(), bias=b.cuda())
+        dx, d_down, d_up = torch.autograd.grad(y, leaves, dy.cuda())
+        others = ids != 1
+        with torch.no_grad():
+            few = E.adapted_projection(leaves[0], w.cuda(), leaves[1], leaves[2], ids.cuda(), bias=b.cuda())
+        for name, got in (("y", y), ("y", few), ("dx", dx)):
+            close(got[others.cuda()], want[name][others], tolerance[name][others], name)
+            assert not torch.isfinite(got[~others.cuda()]).any()
+        for name, got in (("d_down", d_down), ("d_up", d_up)):
+            close(got[[0, 2]], want[name][[0, 2]], tolerance[name][[0, 2]], name)
+        place[1] = kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("inputs,rank", [(40, 5), (40, 20), (300, 5)])
+def test_an_infinite_element_gives_infinities(rows, inputs, rank, dtype):
+    """All weights are positive, so an infinite element of a row makes infinities of its products, and
+    no NaN: not by the padding of the rank and not by the two parts of a low-rank row."""
+    ids, (x, w, down, up, dy) = make(rows, 3, (rows, inputs), (inputs, 70), (3, inputs, rank),
+                                     (3, rank, 70), (rows, 70), dtype=dtype, unknown=0.0)
+    w, down, up, dy = (v.abs() + 0.5 for v in (w, down, up, dy))
+    x[7, 3] = float("inf")
+    t = int(ids[7])
+    leaves = [v.cuda().requires_grad_() for v in (x, w, down, up)]
+    y = E.adapted_projection(*leaves, ids.cuda())
+    with torch.no_grad():
+        few = E.adapted_projection(*leaves, ids.cuda())
+    for got in (y, few):
+        assert bool((got[7] == float("inf")).all()) and bool(torch.isfinite(got[:7]).all())
+        assert bool(torch.isfinite(got[8:]).all())
+    dx, dw, d_down, d_up = torch.autograd.grad(y, leaves, dy.cuda())
+    assert bool(torch.isfinite(dx).all())
+    for got, infinite in ((dw, dw[3]), (d_down, d_down[t, 3]), (d_up, d_up[t])):
+        assert bool((infinite == float("inf")).all())
+        assert int((~torch.isfinite(got)).sum()) == infinite.numel()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_adapted_projection_of_transposed_weights(dtype):
     for rows in (20, 300):
         ids, (x, w, down, up, b, dy) = make(rows, 5, (rows, 36), (36, 44), (5, 36, 6), (5, 6, 44),
@@ -437,6 +493,26 @@ def test_adapted_projection_of_transposed_weights(dtype):
         for name, got in zip(("dx", "dw", "d_down", "d_up", "db"),
                              torch.autograd.grad(y, leaves, dy.cuda())):
             close(got, want[name], tolerance[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inputs", [40, 300])
+def test_scaled_product_at_the_c_boundary(inputs, dtype):
+    """The C structure has a scale for the typed product too: of the product, not of the bias."""
+    ids, (x, w, b) = make(50, 4, (50, inputs), (4, inputs, 36), (4, 36), dtype=dtype)
+    scaled = w.float() * 0.25  # exact
+    want, tolerance = typed_reference(x, scaled.to(dtype), ids, b, dtype=dtype)
+    x, w, b, ids = x.cuda(), w.cuda(), b.cuda(), ids.cuda()
+    plan, y = E.TypePlan(ids, 4), torch.empty((50, 36), dtype=dtype, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for few in (False, True):
+        y.fill_(float("nan"))
+        io, _ = module._product_io(x, inputs, module._weights(w)[1], y, 36, 4, b, None if few else plan,
+                                   ids if few else None, scale=0.25)
+        call = _lib.lib().gn2v_few_rows_product if few else _lib.lib().gn2v_typed_product
+        _lib.check(call(io, stream))
+        close(y, want["y"], tolerance["y"], few)
 
 
 # ---------------------------------------------------------------------- streams, graphs, devices

@@ -206,7 +206,7 @@ def test_infinities_and_nans_stay_in_their_group(codes):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("entries", [1, 300, 1024, 1025, 6000])
+@pytest.mark.parametrize("entries", [1, 300, 512, 513, 1024, 1025, 6000])
 @pytest.mark.parametrize("id_type", [torch.int32, torch.int64])
 def test_the_last_entry_of_a_row_is_kept(entries, id_type):
     rows, width = 500, 40
