@@ -510,8 +510,11 @@ __device__ __forceinline__ bool tile_of_block(uint32_t tiles, uint32_t columns, 
 // elements are contiguous (the transposed product of the backward pass).  ADAPT: tiles are 64
 // consecutive positions of any types; the weights are shared and the rows of every type in the tile
 // get their low-rank part in further steps of the same accumulators.
+// waves per SIMD: what the sums of a run beside those of the tile leave room for
+constexpr int product_waves(int bn, bool adapt) { return adapt && bn == 128 ? 3 : 4; }
+
 template <typename T, int BN, bool WT, bool ADAPT>
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(256, product_waves(BN, ADAPT)) void product_kernel(ProductArgs a) {
     constexpr int E = Tile<T>::kChunk, BK = Tile<T>::kDepth, SLAB = Tile<T>::kSlab;
     constexpr int XS = BK + Tile<T>::kPad;
     constexpr int WS = WT ? XS : BN + (sizeof(T) == 4 ? 4 : 16);
