@@ -3,8 +3,10 @@
 // read back as float32 / bfloat16, and the edge operators read their two rows in this form: a gathered
 // row of 128 columns is 128 + 4 * groups bytes instead of 512.
 //
-//   scale = max(float32(max |x| / largest code value), 2^-90),   code = x / scale rounded ONCE to the
-//   nearest code, ties to even;   value = float32(code * scale).
+//   scale = max(float32(max |x| * float32(1 / largest code value)), 2^-90),   code = x / scale rounded ONCE
+//   to the nearest code, ties to even;   value = float32(code * scale).
+// The scale is off by a last bit or two from the quotient, and the largest |x| / scale then from the largest
+// code value, to which it is rounded all the same.
 // A group that holds an infinity or a NaN gets the scale NaN: all of it reads back as NaN.
 #pragma once
 #include "edge_kernels.h"
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(256) void table_write_kernel(TableView t, const T *
                 if (r[u] < 0 || c >= t.stride) continue;
                 const bool finite = top < 0x7F800000u;
                 constexpr float largest = CODE == kInt8 ? 127.f : 448.f;
-                const float scale = finite ? fmaxf(__uint_as_float(top) / largest, 0x1p-90f) : __builtin_nanf("");
+                const float scale = finite ? fmaxf(__uint_as_float(top) * (1.f / largest), 0x1p-90f) : __builtin_nanf("");
 #pragma unroll
                 for (int w = 0; w < C / 4; ++w)
                     reinterpret_cast<uint32_t *>(t.codes + (uint64_t)r[u] * t.stride + c)[w] =

@@ -510,11 +510,8 @@ __device__ __forceinline__ bool tile_of_block(uint32_t tiles, uint32_t columns, 
 // elements are contiguous (the transposed product of the backward pass).  ADAPT: tiles are 64
 // consecutive positions of any types; the weights are shared and the rows of every type in the tile
 // get their low-rank part in further steps of the same accumulators.
-// waves per SIMD: what the sums of a run beside those of the tile leave room for
-constexpr int product_waves(int bn, bool adapt) { return adapt && bn == 128 ? 3 : 4; }
-
 template <typename T, int BN, bool WT, bool ADAPT>
-__global__ __launch_bounds__(256, product_waves(BN, ADAPT)) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(256, 4) void product_kernel(ProductArgs a) {
     constexpr int E = Tile<T>::kChunk, BK = Tile<T>::kDepth, SLAB = Tile<T>::kSlab;
     constexpr int XS = BK + Tile<T>::kPad;
     constexpr int WS = WT ? XS : BN + (sizeof(T) == 4 ? 4 : 16);
@@ -627,11 +624,10 @@ __global__ __launch_bounds__(256, product_waves(BN, ADAPT)) void product_kernel(
             // bfloat16: 16 runs a tile 381 / 1 593 / 169 / 628 us this way, 423 / 1 584 / 205 / 867 the other;
             // 64 runs 1 183 / 4 160 / 571 / 1 877 and 1 079 / 2 567 / 510 / 1 137.
             if (__popcll(runs) <= 16) {
-                // Few runs: 32 rank columns at a time.  Every run is a product of the whole tile in sums of
-                // its own, which only its rows take: weights that are infinite or NaN reach no row of
-                // another type.  In bfloat16 the low-rank rows enter as a high and a low part.
+                // Few runs: 32 rank columns at a time.  A run is a product in sums of its own, which only its
+                // rows take: weights that are infinite or NaN reach no row of another type.  In bfloat16
+                // the low-rank rows enter as a high and a low part.
                 for (; runs; runs &= runs - 1) {
-                    f32x4 run[MI][NI] = {};
                     const int t = types[__ffsll(runs) - 1];
                     const T *up = (const T *)a.up.data + (int64_t)t * a.up.type;
                     for (int j0 = 0; j0 < a.rank; j0 += 32) {
@@ -653,28 +649,28 @@ __global__ __launch_bounds__(256, product_waves(BN, ADAPT)) void product_kernel(
                         put_w();
                         __syncthreads();
 #pragma unroll
-                        for (int slab = 0; slab < 2; ++slab) {
-                            if (sizeof(T) == 4 && j0 + slab * 16 >= a.rank) break;
-                            Frag<T> xf[MI], wf[NI];
+                        for (int mi = 0; mi < MI; ++mi) {
+                            const bool mine = types[m0 + mi * 16 + (lane & 15)] == t;
+                            if (!__any(mine)) continue;
+                            f32x4 part[NI] = {};
 #pragma unroll
-                            for (int mi = 0; mi < MI; ++mi)
-                                xf[mi].rows(xs, XS, m0 + mi * 16, slab * SLAB, lane);
+                            for (int slab = 0; slab < 2; ++slab) {
+                                if (sizeof(T) == 4 && j0 + slab * 16 >= a.rank) break;
+                                Frag<T> xf;
+                                xf.rows(xs, XS, m0 + mi * 16, slab * SLAB, lane);
 #pragma unroll
-                            for (int ni = 0; ni < NI; ++ni) weights(wf[ni], ni, sizeof(T) == 4 ? slab * SLAB : 0);
+                                for (int ni = 0; ni < NI; ++ni) {
+                                    Frag<T> wf;
+                                    weights(wf, ni, sizeof(T) == 4 ? slab * SLAB : 0);
+                                    part[ni] = mma(wf, xf, part[ni]);
+                                }
+                            }
 #pragma unroll
-                            for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                                for (int ni = 0; ni < NI; ++ni)
-                                    run[mi][ni] = mma(wf[ni], xf[mi], run[mi][ni]);
+                            for (int ni = 0; ni < NI; ++ni)
+                                if (mine) acc[mi][ni] += part[ni];
                         }
                         __syncthreads();
                     }
-#pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-                        if (types[m0 + mi * 16 + (lane & 15)] == t) {
-#pragma unroll
-                            for (int ni = 0; ni < NI; ++ni) acc[mi][ni] += run[mi][ni];
-                        }
                 }
             } else {
                 // Many types, few rows each: every lane adds its row's part from its row's weights.

@@ -450,10 +450,10 @@ typedef struct {
 } gn2v_table8;
 
 /* Quantises values[i] (GN2V_F32 / GN2V_BF16, row stride ldv) into row ids[i] (int32 / int64 by
- * id_bytes; NULL: row i) -- scale = max(max |x| / 127 or 448, 2^-90), codes rounded to the nearest,
- * ties to even; a group with an infinity or a NaN reads back as NaN.  Entries whose id lies outside
- * the table are left out; of several entries of one row the last is kept.  d_owner int32[rows]:
- * scratch, needed with ids and n > GN2V_TABLE_FEW_ENTRIES.  n < 2^31. */
+ * id_bytes; NULL: row i) -- scale = max(max |x| * float32(1 / 127 or 1 / 448), 2^-90), codes rounded
+ * to the nearest, ties to even; a group with an infinity or a NaN reads back as NaN.  Entries whose
+ * id lies outside the table are left out; of several entries of one row the last is kept.  d_owner
+ * int32[rows]: scratch, needed with ids and n > GN2V_TABLE_FEW_ENTRIES.  n < 2^31. */
 #define GN2V_TABLE_FEW_ENTRIES 512u
 int gn2v_table_write(const gn2v_table8 *table, const void *d_values, uint32_t dtype, int64_t ldv,
                      const void *d_ids, uint32_t id_bytes, uint64_t n, int32_t *d_owner, void *stream);

@@ -25,6 +25,12 @@ def e4m3_values():
     return E4M3
 
 
+def scale_of(top, dtype):
+    """The scale of groups whose largest magnitudes are the float32 numbers `top`."""
+    inverse = np.float32(1) / np.float32(CODES[dtype])
+    return np.maximum(np.asarray(top).astype(np.float32) * inverse, np.float32(2.0 ** -90))
+
+
 def quantise(values, dtype, group):
     """(codes as the values they stand for, scales) in 64 bits, by the definition."""
     values = np.asarray(values, dtype=np.float64)
@@ -35,7 +41,7 @@ def quantise(values, dtype, group):
         part = values[:, g * group:(g + 1) * group]
         top = np.abs(part).max(1)
         with np.errstate(invalid="ignore"):
-            scale = np.maximum((top / CODES[dtype]).astype(np.float32), np.float32(2.0 ** -90))
+            scale = scale_of(top, dtype)
         scale[~np.isfinite(top)] = np.nan
         scales[:, g] = scale
         with np.errstate(invalid="ignore"):
@@ -161,11 +167,10 @@ def test_values_next_to_the_borders_of_the_codes(codes):
     """Quotients at, just above and just below the midpoint between two codes, for scales whose
     division is inexact: one rounding, never two."""
     rng = np.random.RandomState(1)
-    largest = CODES[codes]
     rows = []
     for _ in range(400):
         top = np.float32(rng.uniform(0.5, 2) * 2.0 ** rng.randint(-60, 60))
-        scale = np.float64(np.float32(np.float64(top) / largest))
+        scale = np.float64(scale_of(top, codes))
         if codes == torch.int8:
             middle = rng.randint(0, 126, 15) + 0.5
         else:
