@@ -510,6 +510,13 @@ __device__ __forceinline__ bool tile_of_block(uint32_t tiles, uint32_t columns, 
 // elements are contiguous (the transposed product of the backward pass).  ADAPT: tiles are 64
 // consecutive positions of any types; the weights are shared and the rows of every type in the tile
 // get their low-rank part in further steps of the same accumulators.
+//
+// One stage of the inner axis is multiplied while the next one's loads are under way; four workgroups per CU
+// take turns at the barriers.  float32 is bound by the matrix instructions (300 000 rows of 512 -> 512: 1 423
+// us, 0.72 of the 154 TFLOP/s that a large product reaches), bfloat16 by what the fragments take from LDS, 6 KB
+// for eight 16-cycle instructions (368 us, 427 TFLOP/s).  Tiles of 128 rows, eight waves and two buffers an
+// operand gave the same in bfloat16 (365 us) and in float32 left too few workgroups to hide a barrier
+// behind another (400 000 rows of 256 -> 256: 712 us instead of 506).
 template <typename T, int BN, bool WT, bool ADAPT>
 __global__ __launch_bounds__(256, 4) void product_kernel(ProductArgs a) {
     constexpr int E = Tile<T>::kChunk, BK = Tile<T>::kDepth, SLAB = Tile<T>::kSlab;
@@ -728,7 +735,10 @@ __global__ __launch_bounds__(256, 4) void product_kernel(ProductArgs a) {
 //
 // What a CU can have under way towards its L2 bounds both the rows and the weights (some 20 KB a
 // microsecond): weights are therefore read once per workgroup, whole lines at a time, and dealt out
-// through the LDS of the rows.
+// through the LDS of the rows.  2.4 M bfloat16 rows of 128 -> 128, 16 types: 248 us, 5.0 TB/s (450 us in the
+// kernel above); 169 343 float32 rows of 128 -> 128, 40 types: 70 us, where the bytes take 36 us and the
+// matrix instructions 36 us, and a workgroup's five or six tiles leave a quarter of the time to its start
+// and to the last tile.
 constexpr int kFusedRank = 16;
 constexpr int kNarrowThreads = 512;
 
@@ -985,7 +995,9 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
 
 // --------------------------------------------------------------------------------- few rows
 // One workgroup per row and 64 columns: lanes read 16 bytes of a weight row each, the workgroup's
-// 256 / (64 / kChunk) row groups split the inner axis and are joined in LDS.  No plan, one launch.
+// 256 / (64 / kChunk) row groups split the inner axis and are joined in LDS.  No plan, one launch.  Bound by
+// latency while there are fewer workgroups than CUs (64 rows of 128 -> 128 float32: 3.8 us), then by the
+// weights that every row reads through L2 (512 rows of 512 -> 256: 268 MB in 15.7 us).
 constexpr int kFewDepth = 4096;  // inner elements a workgroup keeps in LDS
 constexpr int kMaxRank = 64;
 
@@ -1083,7 +1095,8 @@ __global__ __launch_bounds__(256) void few_rows_kernel(FewArgs a) {
 // a type that began before it in its first slot, those of a type that goes on behind it in its second; a
 // second launch joins them in order (no atomics: the same bits in every run).  Either operand may be
 // float32 rows at their positions (the low-rank rows), which enter bfloat16 products as a high and a
-// low part.
+// low part.  Both operands lie in LDS with the rows as the inner axis, which is what a transposed read
+// (bfloat16) or four words (float32) take.  Bound by HBM: 2.4 M bfloat16 rows of 128 x 128 262 us, 4.7 TB/s.
 enum GradSpan : int { kKnownTiles = 0, kRowBlocks = 1, kAllTiles = 2 };
 
 struct GradArgs {
@@ -1306,8 +1319,11 @@ __global__ __launch_bounds__(256, grad_waves(MI, NI)) void grad_kernel(GradArgs 
 // All gradients of the adapted form at once, for rows and outputs of up to 128 elements and ranks of up
 // to 16: d_down[t] = sum of x[r]^T back[r], d_up[t] = sum of low[r]^T dy[r] over the rows of type t, and
 // (WANT_W) dW = sum of x[r]^T dy[r], db = sum of dy[r] over all rows.  The low-rank rows are further
-// columns of the two LDS tiles, so that x and dy are read once instead of twice.  `types` has the sums
-// per type (dw: d_down, db: d_up), `all` those of the shared weights.
+// columns of the two LDS tiles, so that x and dy are read once instead of three times (1 M bfloat16 rows
+// of 128 x 128, rank 16: 205 us with the joins instead of 331).  `types` has the sums per type (dw: d_down,
+// db: d_up), `all` those of the shared weights.  640 MB in 195 us, 3.3 TB/s: waves wait 0.69 of their cycles,
+// 0.02 for LDS, so what bounds it is how many rows are under way -- 32 a workgroup, as many workgroups as
+// fit the LDS.
 struct AdaptedGradArgs {
     GradArgs types, all;
     const float *low, *back;  // [position][rank]
