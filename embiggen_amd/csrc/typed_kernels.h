@@ -778,7 +778,10 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
     const uint32_t ranges = min(a.ranges, (uint32_t)tiles);
     if (range >= ranges) return;
     const int first = range_first(range, tiles, ranges), last = range_first(range + 1, tiles, ranges);
-    const int wn = wave % WAVES_N, m0 = wave / WAVES_N * MI * 16, nb = (int)column * BN, n0 = nb + wn * 16 * NI;
+    // Waves behind the last column have nothing to multiply; which they are takes turns among the workgroups
+    // of a CU, and so do the SIMDs that they leave.
+    const int turn = (wave + (int)(range >> 8)) & 7;
+    const int wn = turn % WAVES_N, m0 = turn / WAVES_N * MI * 16, nb = (int)column * BN, n0 = nb + wn * 16 * NI;
     const int n = n0 + 4 * NI * (lane >> 4);  // the lane's 4 * NI output columns
     const int unknown = (int)a.plan.types;
     u32x4 xr[XL];
@@ -909,7 +912,7 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
             if (ends && t + 2 < last && tid < 64) id_ahead = id_of(ahead2);
             if (!ends || t + 1 < last) fetch(ends ? ids[next] : id + r0 + ROWS);
             // 16-row blocks of this wave that hold rows
-            const int live = (count - r0 - m0 + 15) >> 4;
+            const int live = n0 < a.N ? (count - r0 - m0 + 15) >> 4 : 0;
             f32x4 acc[MI][NI] = {};
             if (ADAPT || known) {
 #pragma unroll

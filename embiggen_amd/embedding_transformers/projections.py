@@ -8,8 +8,10 @@ Both run in hand-written kernels that read the rows where they are: a *plan* (``
 order of the rows by type, and no sorted copy of them is made.  Both can be differentiated; gradients
 are summed in a fixed order, so a run gives the same bits every time.
 """
+import collections
 import ctypes as C
 import functools
+import struct
 from typing import Optional, Union
 
 from .. import _lib
@@ -40,6 +42,9 @@ def _check_rows(name: str, x, dims: int):
 
 
 def _check_like(name: str, tensor, shape, x):
+    if (isinstance(tensor, _torch().Tensor) and tensor.shape == shape and tensor.dtype == x.dtype
+            and tensor.device == x.device):
+        return
     _check_rows(name, tensor, len(shape))
     if tuple(tensor.shape) != tuple(shape):
         raise ValueError(f"The provided {name} should have shape {tuple(shape)}, but we got "
@@ -133,17 +138,25 @@ class TypePlan:
 
 def _row_stride(x):
     """(tensor, elements between rows): the tensor itself where its rows lie apart."""
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        if x.shape[0] == 1 and (x.shape[1] == 1 or x.stride(1) == 1):
-            return x, x.shape[1]
-        x = x.contiguous()
-    return x, max(x.stride(0), x.shape[1])
+    (rows, width), (apart, inner) = x.shape, x.stride()
+    if width > 1 and inner != 1 or apart < width:
+        if rows != 1 or width > 1 and inner != 1:
+            x = x.contiguous()
+        return x, width
+    return x, apart
+
+
+# gn2v_weights (include/gn2v_internal.h) by its fields
+_View = collections.namedtuple("_View", "d_data type_stride inner outer")
 
 
 def _weights(w, rows_contiguous: bool = False):
-    """(tensor, gn2v_weights) of [inputs, outputs] or [types, inputs, outputs] weights: as they are
+    """(tensor, _View) of [inputs, outputs] or [types, inputs, outputs] weights: as they are
     where one of the two last strides is 1 (``rows_contiguous``: the last one), else a copy."""
-    inner, outer = w.stride(-2), w.stride(-1)
+    strides = w.stride()
+    inner, outer = strides[-2:]
+    if outer == 1:
+        return w, _View(w.data_ptr(), strides[0] if len(strides) == 3 else 0, inner, 1)
     if w.shape[-1] == 1:
         outer = 1
     elif w.shape[-2] == 1 and outer != 1 and not rows_contiguous:
@@ -151,18 +164,20 @@ def _weights(w, rows_contiguous: bool = False):
     if outer != 1 and (rows_contiguous or inner != 1):
         w = w.contiguous()
         inner, outer = w.stride(-2), 1
-    return w, _lib.Weights(w.data_ptr(), w.stride(0) if w.dim() == 3 else 0, inner, outer)
+    return w, _View(w.data_ptr(), w.stride(0) if w.dim() == 3 else 0, inner, outer)
 
 
 def _transposed(view):
-    return _lib.Weights(view.d_data, view.type_stride, view.outer, view.inner)
+    return _View(view.d_data, view.type_stride, view.outer, view.inner)
 
 
 def _dtype(x) -> int:
     return 0 if x.dtype == _torch().float32 else 1
 
 
-_NO_WEIGHTS = _lib.Weights()
+_NO_WEIGHTS = _View(0, 0, 0, 0)
+# gn2v_product_io as it lies in memory: packed at once, in a quarter of the time its fields take one by one
+_PRODUCT = struct.Struct("IIQIIPqPqqqPqPqPPIIfIPqqqPqqqP")
 
 
 def _product_io(x, ldx, weight, y, outputs, n_types, bias=None, plan=None, types=None, rank=0,
@@ -170,17 +185,19 @@ def _product_io(x, ldx, weight, y, outputs, n_types, bias=None, plan=None, types
     """(gn2v_product_io, what has to outlive the call)."""
     bias_stride = 0
     if bias is not None:
-        if bias.shape[-1] > 1 and bias.stride(-1) != 1:
+        strides = bias.stride()
+        if strides[-1] != 1 and bias.shape[-1] > 1:
             bias = bias.contiguous()
-        bias_stride = bias.stride(0) if bias.dim() == 2 else 0
+            strides = bias.stride()
+        bias_stride = strides[0] if len(strides) == 2 else 0
     if types is not None:
         types = types.contiguous()
-    return _lib.ProductIO(
-        _dtype(x), n_types, x.shape[0], x.shape[1], outputs, x.data_ptr(), ldx, weight,
-        None if bias is None else bias.data_ptr(), bias_stride, y.data_ptr(), y.shape[1],
-        None if plan is None else plan._words.data_ptr(),
-        None if types is None else types.data_ptr(), 0 if types is None else types.element_size(),
-        rank, scale, low_rank_rows, down, up, None if low is None else low.data_ptr()), (bias, types)
+    return _lib.ProductIO.from_buffer_copy(_PRODUCT.pack(
+        _dtype(x), n_types, *x.shape, outputs, x.data_ptr(), ldx, *weight,
+        0 if bias is None else bias.data_ptr(), bias_stride, y.data_ptr(), y.shape[1],
+        0 if plan is None else plan._words.data_ptr(),
+        0 if types is None else types.data_ptr(), 0 if types is None else types.element_size(),
+        rank, scale, low_rank_rows, *down, *up, 0 if low is None else low.data_ptr())), (bias, types)
 
 
 def _typed_product(x, ldx, weight, plan, outputs, bias=None):
@@ -279,8 +296,9 @@ def _few_rows(x, plan, types, weight, number_of_types, bias=None, down=None, up=
     if (not 0 < rows <= FEW_ROWS or inputs > _lib.FEW_ROWS_DEPTH
             or rows * inputs * outputs * x.element_size() > FEW_BYTES):
         return None
-    if any(w is not None and w.shape[-1] > 1 and w.stride(-1) != 1 for w in (weight, down, up)):
-        return None  # transposed weights would be copied whole
+    for w in (weight,) if down is None else (weight, down, up):
+        if w.stride(-1) != 1 and w.shape[-1] > 1:
+            return None  # transposed weights would be copied whole
     x, ldx = _row_stride(x)
     weight, view = _weights(weight, True)
     y = _torch().empty((rows, outputs), dtype=x.dtype, device=x.device)
@@ -412,7 +430,10 @@ def _check_types(types, x, number_of_types: int):
 
 
 def _wants_gradient(*tensors) -> bool:
-    return _torch().is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for tensor in tensors:
+        if tensor is not None and tensor.requires_grad:
+            return _torch().is_grad_enabled()
+    return False
 
 
 def typed_projection(x, weight, types: Union["TypePlan", "object"], bias=None):

@@ -173,6 +173,21 @@ def test_refusals_at_the_c_boundary():
     assert L.gn2v_typed_gradient_temp(C.byref(g), C.byref(a)) == 1
 
 
+def test_the_packed_structure_has_its_fields():
+    x, y = torch.zeros(3, 5), torch.zeros(3, 7)
+    w, b = torch.zeros(2, 5, 7), torch.zeros(2, 7)
+    down, up, low, ids = torch.zeros(2, 5, 4), torch.zeros(2, 4, 7), torch.zeros(3, 4), torch.zeros(3, dtype=torch.int64)
+    views = [module._weights(t)[1] for t in (w, down, up)]
+    io, _ = module._product_io(x, 5, views[0], y, 7, 2, b, None, ids, 4, 0.5, 1, views[1], views[2], low)
+    assert module._PRODUCT.size == C.sizeof(_lib.ProductIO)
+    assert (io.dtype, io.n_types, io.rows, io.inputs, io.outputs, io.ldx, io.ldy) == (0, 2, 3, 5, 7, 5, 7)
+    assert (io.d_x, io.d_y, io.d_bias, io.d_types, io.d_low, io.d_plan) == (
+        x.data_ptr(), y.data_ptr(), b.data_ptr(), ids.data_ptr(), low.data_ptr(), None)
+    assert (io.bias_stride, io.type_bytes, io.rank, io.scale, io.low_rank_rows) == (7, 8, 4, 0.5, 1)
+    for view, field in zip(views, (io.weight, io.down, io.up)):
+        assert tuple(view) == (field.d_data, field.type_stride, field.inner, field.outer)
+
+
 def test_weight_views_need_no_copies():
     w = torch.zeros(3, 4, 5)
     same, view = module._weights(w)
