@@ -178,6 +178,8 @@ def _dtype(x) -> int:
 _NO_WEIGHTS = _View(0, 0, 0, 0)
 # gn2v_product_io as it lies in memory: packed at once, in a quarter of the time its fields take one by one
 _PRODUCT = struct.Struct("IIQIIPqPqqqPqPqPPIIfIPqqqPqqqP")
+_GRADIENT = struct.Struct("IIQIIPPqqIIIIPPPPQ")
+_ADAPTED_GRADIENT = struct.Struct("IIQIIIIPPqqPPPPPPPPQ")
 
 
 def _product_io(x, ldx, weight, y, outputs, n_types, bias=None, plan=None, types=None, rank=0,
@@ -248,7 +250,7 @@ def _gradient_bytes(adapted: bool, *sizes) -> int:
 
 
 def _ptr(tensor):
-    return None if tensor is None else tensor.data_ptr()
+    return 0 if tensor is None else tensor.data_ptr()
 
 
 def _gradient(x, dy, plan, dw, db):
@@ -260,8 +262,9 @@ def _gradient(x, dy, plan, dw, db):
              dy.shape[1])
     need = _gradient_bytes(False, *sizes)
     temp = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    io = _lib.GradientIO(*sizes, x.data_ptr(), dy.data_ptr(), ldx, ldy, 0, 0, 0, 0,
-                         plan._words.data_ptr(), _ptr(dw), _ptr(db), temp.data_ptr(), need)
+    io = _lib.GradientIO.from_buffer_copy(_GRADIENT.pack(
+        *sizes, x.data_ptr(), dy.data_ptr(), ldx, ldy, 0, 0, 0, 0, plan._words.data_ptr(), _ptr(dw),
+        _ptr(db), temp.data_ptr(), need))
     _lib.check(_lib.lib().gn2v_typed_gradient(io, _stream(dy)))
 
 
@@ -271,12 +274,12 @@ def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
     x, ldx = _row_stride(x)
     dy, ldy = _row_stride(dy)
     sizes = (_dtype(x), plan.number_of_types, x.shape[0], x.shape[1], dy.shape[1], rank)
-    parts = (d_down, d_up, dw, db)
-    need = _gradient_bytes(True, *sizes, *(t is not None for t in parts))
+    need = _gradient_bytes(True, *sizes, d_down is not None, d_up is not None, dw is not None,
+                           db is not None)
     temp = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    io = _lib.AdaptedGradientIO(*sizes, 0, x.data_ptr(), dy.data_ptr(), ldx, ldy, _ptr(low),
-                                _ptr(back), plan._words.data_ptr(), *(_ptr(t) for t in parts),
-                                temp.data_ptr(), need)
+    io = _lib.AdaptedGradientIO.from_buffer_copy(_ADAPTED_GRADIENT.pack(
+        *sizes, 0, x.data_ptr(), dy.data_ptr(), ldx, ldy, _ptr(low), _ptr(back),
+        plan._words.data_ptr(), _ptr(d_down), _ptr(d_up), _ptr(dw), _ptr(db), temp.data_ptr(), need))
     _lib.check(_lib.lib().gn2v_adapted_gradient(io, _stream(dy)))
 
 

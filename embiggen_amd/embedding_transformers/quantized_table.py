@@ -166,28 +166,29 @@ class QuantizedTable:
         if not isinstance(values, torch.Tensor) or values.dim() != 2:
             raise ValueError("The values should be a two-dimensional tensor.")
         kind = _value_type(values.dtype)
-        if values.shape[1] != self.embedding_size or values.device != self.device:
+        n, width = values.shape
+        if width != self.embedding_size or values.device != self._codes.device:
             raise ValueError(f"The values should be rows of {self.embedding_size} columns on "
                              f"{self.device}, but we got shape {tuple(values.shape)} on "
                              f"{values.device}.")
-        n = values.shape[0]
         if rows is None:
             if n > len(self):
                 raise ValueError(f"{n} rows do not fit a table of {len(self)}.")
         else:
-            rows = _ids(rows, self.device, "rows")
-            if rows.numel() != n:
+            rows = _ids(rows, values.device, "rows")
+            if rows.shape[0] != n:
                 raise ValueError(f"There are {n} values, but rows for {rows.numel()}.")
-        values = values.detach()
-        if values.stride(1) != 1 or values.stride(0) < values.shape[1]:
-            values = values.contiguous()
+        apart, inner = values.stride()
+        if inner != 1 or apart < self.embedding_size:
+            values = values.detach().contiguous()
+            apart = values.stride(0)
         owner = None
         if rows is not None and n > _lib.TABLE_FEW_ENTRIES:
             owner = torch.empty(len(self), dtype=torch.int32, device=self.device)
         _lib.check(_lib.lib().gn2v_table_write(
-            self._io, values.data_ptr(), kind, max(values.stride(0), values.shape[1]),
+            self._io, values.data_ptr(), kind, max(apart, self.embedding_size),
             None if rows is None else rows.data_ptr(), 0 if rows is None else rows.element_size(), n,
-            None if owner is None else owner.data_ptr(), _stream(self.codes)))
+            None if owner is None else owner.data_ptr(), _stream(self._codes)))
 
     def read(self, rows=None, dtype=None):
         """The rows ``rows`` (int32 / int64; by default all) as a float32 (or bfloat16: ``dtype``)
@@ -196,13 +197,13 @@ class QuantizedTable:
         dtype = torch.float32 if dtype is None else dtype
         kind = _value_type(dtype)
         if rows is not None:
-            rows = _ids(rows, self.device, "rows")
-        n = len(self) if rows is None else rows.numel()
-        out = torch.empty((n, self.embedding_size), dtype=dtype, device=self.device)
+            rows = _ids(rows, self._codes.device, "rows")
+        n = len(self) if rows is None else rows.shape[0]
+        out = torch.empty((n, self.embedding_size), dtype=dtype, device=self._codes.device)
         _lib.check(_lib.lib().gn2v_table_read(
             self._io, None if rows is None else rows.data_ptr(),
             0 if rows is None else rows.element_size(), n, out.data_ptr(), kind,
-            self.embedding_size, _stream(self.codes)))
+            self.embedding_size, _stream(self._codes)))
         return out
 
 

@@ -179,7 +179,16 @@ def test_the_packed_structure_has_its_fields():
     down, up, low, ids = torch.zeros(2, 5, 4), torch.zeros(2, 4, 7), torch.zeros(3, 4), torch.zeros(3, dtype=torch.int64)
     views = [module._weights(t)[1] for t in (w, down, up)]
     io, _ = module._product_io(x, 5, views[0], y, 7, 2, b, None, ids, 4, 0.5, 1, views[1], views[2], low)
-    assert module._PRODUCT.size == C.sizeof(_lib.ProductIO)
+    for packed, structure in ((module._PRODUCT, _lib.ProductIO), (module._GRADIENT, _lib.GradientIO),
+                              (module._ADAPTED_GRADIENT, _lib.AdaptedGradientIO)):
+        assert packed.size == C.sizeof(structure)
+        image = bytes(range(packed.size))
+        filled = structure.from_buffer_copy(image)
+        fields = []
+        for name, _ in structure._fields_:
+            value = getattr(filled, name)
+            fields += [getattr(value, f) for f, _ in value._fields_] if isinstance(value, _lib.Weights) else [value]
+        assert packed.unpack(image) == tuple(fields)
     assert (io.dtype, io.n_types, io.rows, io.inputs, io.outputs, io.ldx, io.ldy) == (0, 2, 3, 5, 7, 5, 7)
     assert (io.d_x, io.d_y, io.d_bias, io.d_types, io.d_low, io.d_plan) == (
         x.data_ptr(), y.data_ptr(), b.data_ptr(), ids.data_ptr(), low.data_ptr(), None)
