@@ -748,7 +748,14 @@ constexpr int narrow_rows(int slabs, bool adapt) { return slabs == 8 && adapt ? 
 // 16-column blocks per wave.  Two, whose columns a lane holds in turn, make the stores of a bfloat16 row
 // 64 bytes long instead of 32 (a launch of 2.4 M rows of 128: 250 us instead of 299); longer rows leave
 // no registers for it, and float rows need no help.
-constexpr int narrow_blocks(int size, int slabs) { return size == 2 && slabs < 8 ? 2 : 1; }
+constexpr int narrow_blocks(int size, int slabs) { return size == 2 && slabs < 6 ? 2 : 1; }
+
+// Slabs of weights that go through LDS at a time, where it has room for `fit` of them.
+constexpr int narrow_step(int slabs, int fit) {
+    int step = slabs;
+    while (step > fit) step = step % 2 ? 1 : step / 2;
+    return step;
+}
 
 template <typename T, int SLABS, int BN, bool WT, bool ADAPT>
 __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(ProductArgs a) {
@@ -763,7 +770,7 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
     constexpr int WS = BN + (sizeof(T) == 4 ? 4 : 16);
     constexpr int LDS_X = 2 * ROWS * XS, LDS_W = LDS_X > 17408 / (int)sizeof(T) ? LDS_X : 17408 / (int)sizeof(T);
     constexpr int FIT = LDS_W / (WT ? BN * (SLAB + Tile<T>::kPad) : SLAB * WS);
-    constexpr int STEP = FIT >= SLABS ? SLABS : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+    constexpr int STEP = narrow_step(SLABS, FIT);
     constexpr int WTS = STEP * SLAB + Tile<T>::kPad;
     static_assert((WT ? BN * WTS : STEP * SLAB * WS) <= LDS_W || STEP == 1, "weights in passes");
     __shared__ __align__(16) T xs[LDS_W];

@@ -262,7 +262,7 @@ SHAPES = [  # rows, types, inputs, outputs
     (1, 1, 1, 1), (1, 3, 128, 128), (7, 2, 3, 5), (48, 7, 100, 100), (64, 1, 32, 32),
     (65, 3, 33, 31), (129, 5, 64, 65), (200, 300, 17, 129), (1025, 4, 100, 71),
     (3001, 9, 130, 96), (5000, 3, 256, 200), (2049, 1, 128, 128), (300, 4, 300, 1), (300, 4, 1, 300),
-    (700, 3, 513, 140), (90, 2, 5000, 10),
+    (700, 3, 513, 140), (90, 2, 5000, 10), (1500, 3, 90, 100), (1400, 3, 65, 60), (1300, 4, 160, 150),
 ]
 
 
@@ -392,6 +392,9 @@ ADAPTED = [  # rows, types, inputs, outputs, rank, skew
     (2100, 900, 50, 64, 4, False), (3000, 6, 200, 32, 32, True), (300, 4, 40, 1, 20, False),
     (300, 4, 1, 40, 20, False), (150, 3, 1, 1, 1, False), (400, 3, 300, 1, 1, False),
     (400, 3, 1, 300, 1, False), (500, 4, 300, 260, 16, False), (260, 5, 140, 130, 9, True),
+    (1600, 7, 90, 90, 8, True), (1200, 3, 170, 80, 16, False),
+    # rows of 300 elements: some runs of one type a tile, and nearly as many types as rows
+    (800, 100, 300, 40, 8, False), (600, 500, 300, 70, 20, False),
 ]
 
 
