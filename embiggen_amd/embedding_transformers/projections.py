@@ -6,7 +6,9 @@ an adapter.  The reference's classifiers treat types as one-hot columns beside t
 (embiggen/embedding_transformers/graph_transformer.py:196-243); here every type has weights of its own.
 Both run in hand-written kernels that read the rows where they are: a *plan* (``TypePlan``) holds the
 order of the rows by type, and no sorted copy of them is made.  Both can be differentiated; gradients
-are summed in a fixed order, so a run gives the same bits every time.
+are summed in a fixed order, so a run gives the same bits every time.  Calls are made on the current
+stream and can be captured into a graph, the plan's among them; a backward pass that is captured takes
+leaves that no eager graph holds at the time.
 """
 import collections
 import ctypes as C
