@@ -5,8 +5,8 @@ their node or edge type, or through one shared projection plus a low-rank correc
 an adapter.  The reference's classifiers treat types as one-hot columns beside the embedding
 (embiggen/embedding_transformers/graph_transformer.py:196-243); here every type has weights of its own.
 Both run in hand-written kernels that read the rows where they are: a *plan* (``TypePlan``) holds the
-order of the rows by type, and no sorted copy of them is made.  Both can be differentiated; gradients
-are summed in a fixed order, so a run gives the same bits every time.  Calls are made on the current
+order of the rows by type, and no sorted copy of them is made.  Both can be differentiated backwards, once
+(forward-mode derivatives are refused); gradients are summed in a fixed order, so a run gives the same bits every time.  Calls are made on the current
 stream and can be captured into a graph, the plan's among them; a backward pass that is captured takes
 leaves that no eager graph holds at the time.
 """
@@ -344,6 +344,7 @@ def _functions():
 
         @once
         def backward(ctx, dy):
+            _refuse_tangents(dy)
             x, weight = ctx.saved_tensors
             plan = ctx.plan
             dx = dw = db = None
@@ -376,6 +377,7 @@ def _functions():
 
         @once
         def backward(ctx, dy):
+            _refuse_tangents(dy)
             x, weight, down, up, low = ctx.saved_tensors
             plan, wanted = ctx.plan, ctx.needs_input_grad
             dx = dw = d_down = d_up = db = None
@@ -434,6 +436,17 @@ def _check_types(types, x, number_of_types: int):
         raise ValueError(f"The types are on {device}, but the rows on {x.device}.")
 
 
+def _refuse_tangents(*tensors):
+    """The kernels see a tensor's values alone: a forward-mode tangent would be lost without a word."""
+    forward_ad = _torch().autograd.forward_ad
+    if forward_ad._current_level < 0:  # nobody differentiates forwards; unpacking costs 0.3 us a tensor
+        return
+    for tensor in tensors:
+        if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+            raise NotImplementedError("The projections have no forward-mode derivatives, but one of the "
+                                      "provided tensors has a tangent.")
+
+
 def _wants_gradient(*tensors) -> bool:
     for tensor in tensors:
         if tensor is not None and tensor.requires_grad:
@@ -460,7 +473,7 @@ def typed_projection(x, weight, types: Union["TypePlan", "object"], bias=None):
     Returns
     ------------------
     [rows, outputs] of the rows' type; products are summed in float32 and rounded once.  Differentiable
-    in ``x``, ``weight`` and ``bias``.
+    in ``x``, ``weight`` and ``bias`` (backwards, once; a tensor with a forward-mode tangent is refused).
     """
     _check_rows("rows", x, 2)
     _check_rows("weight", weight, 3)
@@ -472,6 +485,7 @@ def typed_projection(x, weight, types: Union["TypePlan", "object"], bias=None):
         _check_like("bias", bias, (n_types, outputs), x)
     _check_types(types, x, n_types)
     _check_device(x)
+    _refuse_tangents(x, weight, bias)
     plan = types if isinstance(types, TypePlan) else None
     if not _wants_gradient(x, weight, bias):
         y = _few_rows(x, plan, types, weight, n_types, bias)
@@ -503,8 +517,8 @@ def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], 
 
     Returns
     ------------------
-    [rows, outputs] of the rows' type.  Differentiable in every tensor but the types; leave the
-    gradient of ``weight`` and ``bias`` off to train the corrections alone.
+    [rows, outputs] of the rows' type.  Differentiable in every tensor but the types, as
+    ``typed_projection`` is; leave the gradient of ``weight`` and ``bias`` off to train the corrections alone.
     """
     _check_rows("rows", x, 2)
     _check_rows("weight", weight, 2)
@@ -525,6 +539,7 @@ def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], 
         _check_like("bias", bias, (outputs,), x)
     _check_types(types, x, n_types)
     _check_device(x)
+    _refuse_tangents(x, weight, down, up, bias)
     plan = types if isinstance(types, TypePlan) else None
     scale = float(scale)
     if not _wants_gradient(x, weight, down, up, bias):
