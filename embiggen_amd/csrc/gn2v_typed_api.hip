@@ -16,6 +16,9 @@ namespace {
 
 constexpr uint64_t kMaxRows = (1ull << 31) - (1ull << 20);  // positions are int32
 
+// A launch holds fewer than 2^32 threads along an axis.
+constexpr uint64_t max_blocks(uint64_t threads) { return 0xFFFFFFFFull / threads; }
+
 // the plan's words, and the stripes its rows are counted in
 struct PlanSizes {
     uint64_t words, temp;
@@ -205,8 +208,10 @@ bool is_narrow(uint32_t dtype, uint32_t inputs) { return inputs <= (dtype == GN2
 
 template <bool ADAPT>
 int launch_product(uint32_t dtype, const gn2v::ProductArgs &a, bool wt, bool narrow, hipStream_t s) {
-    if ((product_tiles(a, false) + 7) / 8 * 8 * ((a.N + 31) / 32) > 0x7FFFFFFFull)
-        return fail("too many tiles for one launch");
+    // one workgroup per tile and block of columns, as launch_product_bn chooses it; narrow rows: resident ones
+    const uint64_t bn = a.N <= 32 ? 32 : a.N <= 64 ? 64 : 128;
+    if (!narrow && (product_tiles(a, ADAPT) + 7) / 8 * 8 * ((a.N + bn - 1) / bn) > max_blocks(256))
+        return fail("too many rows and columns for one launch: at most 2^24 tiles of 64 rows x 128 columns");
     if (narrow) {
         if (dtype == GN2V_F32)
             wt ? launch_narrow<float, true, ADAPT>(a, s) : launch_narrow<float, false, ADAPT>(a, s);
@@ -267,7 +272,11 @@ template <typename T>
 void launch_join(const gn2v::GradArgs &a, uint32_t types, hipStream_t s) {
     // few types lie in many ranges each: sixteen waves share them, four where there are many types
     const uint64_t blocks = types * (uint64_t)((a.stride + 255) / 256);
-    hipLaunchKernelGGL((gn2v::grad_join_kernel<T>), dim3((unsigned)blocks), dim3(types >= 64 ? 256 : 1024), 0, s, a);
+    const unsigned threads = types >= 64 ? 256 : 1024;
+    // 2^30 sums with sixteen waves, 2^32 with four fill a launch
+    for (uint64_t first = 0; first < blocks; first += max_blocks(threads))
+        hipLaunchKernelGGL((gn2v::grad_join_kernel<T>), dim3((unsigned)std::min(blocks - first, max_blocks(threads))),
+                           dim3(threads), 0, s, a, first);
 }
 
 // The adapted form's gradients in one pass over the rows: small enough for one block of sums.  The
@@ -627,8 +636,7 @@ int gn2v_typed_gradient(const gn2v_gradient_io *io, void *stream) {
     const uint64_t kb = std::max<uint64_t>(1, (io->inputs + g.bm - 1) / g.bm), nb = (io->outputs + g.bn - 1) / g.bn;
     const uint64_t blocks = (g.ranges + 7ull) / 8 * 8 * kb * nb;
     const uint32_t types = io->shared ? 1 : io->n_types;
-    if (blocks > 0x7FFFFFFFull || types * ((g.stride + 255) / 256) > 0x7FFFFFFFull)
-        return fail("too many blocks for one launch");
+    if (blocks > max_blocks(256)) return fail("too many inputs and outputs for one launch");
     DeviceGuard guard(DeviceGuard::of_pointer(io->d_dw ? io->d_dw : io->d_db));
     hipStream_t s = (hipStream_t)stream;
     const uint32_t size = size_of(io->dtype);

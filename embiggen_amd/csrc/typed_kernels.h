@@ -1550,14 +1550,15 @@ __global__ __launch_bounds__(256, adapted_grad_groups(sizeof(T))) void adapted_g
 }
 
 // Joins the ranges of a type in their order: the workgroup's waves sum an equal share of them each, 256
-// elements at a time.  Types without rows get zeros; types inside one range are done.
+// elements at a time.  Types without rows get zeros; types inside one range are done.  `first_block`: of the
+// workgroups of all types, where this launch's begin.
 template <typename T>
-__global__ __launch_bounds__(1024) void grad_join_kernel(GradArgs a) {
+__global__ __launch_bounds__(1024) void grad_join_kernel(GradArgs a, uint64_t first_block) {
     __shared__ f32x4 part[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t blocks = (a.stride + 255) / 256;
-    const int type = (int)(blockIdx.x / blocks);
-    const int64_t at = (int64_t)(blockIdx.x % blocks) * 256 + lane * 4;
+    const uint64_t blocks = (uint64_t)(a.stride + 255) / 256, block = first_block + blockIdx.x;
+    const int type = (int)(block / blocks);
+    const int64_t at = (int64_t)(block % blocks) * 256 + lane * 4;
     const int tiles = a.plan.rows ? grad_tiles(a) : 0;  // no rows: no plan
     const int type_first = a.shared || !tiles ? 0 : a.plan.tile_first[type];
     const int type_last = a.shared || !tiles ? tiles : a.plan.tile_first[type + 1];

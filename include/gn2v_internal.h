@@ -342,7 +342,8 @@ int gn2v_touch_rows(float *d_table, uint32_t ld, const uint32_t *d_ids, uint64_t
  * the 0xFFFFFFFF of gn2v_graph_set_types read as int32 -- is an unknown type, and its rows come
  * last.  d_plan int32[plan_words]: order[rows], row_types[rows] (by position), offsets[n_types + 2],
  * and the types' first tiles (of 64 rows) likewise.  d_temp int32[temp_words] is free again once the launch is over.
- * rows <= 2^31 - 2^20, 1 <= n_types <= GN2V_MAX_TYPES. */
+ * rows <= 2^31 - 2^20, 1 <= n_types <= GN2V_MAX_TYPES.  A product of more than 2^24 tiles of 64 rows x 32, 64
+ * or 128 columns (low-rank rows: 2^30 rows) is refused: it does not fit one launch. */
 #define GN2V_MAX_TYPES 32768u
 #define GN2V_MAX_RANK 64u
 int gn2v_type_plan_words(uint64_t rows, uint32_t n_types, uint64_t *plan_words, uint64_t *temp_words);

@@ -1,10 +1,13 @@
 """What the projections refuse, and how they behave at the ends of what they allow: forward-mode
 derivatives, many tiles a workgroup, sizes that pass 32 bits, other streams."""
+import ctypes as C
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import embiggen_amd as E
+from embiggen_amd import _lib
 from embiggen_amd.embedding_transformers import projections as module
 
 
@@ -57,3 +60,40 @@ def test_forward_mode_derivatives_are_refused(on_the_cpu, rows):
         twice = torch.autograd.grad(run(leaves), leaves, torch.ones(rows, 5).requires_grad_(), create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             twice[0].sum().backward()
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256, one per 64 rows of the low-rank rows."""
+    rows = (1 << 30) + (1 << 20)
+    io = _lib.ProductIO(dtype=1, n_types=2, rows=rows, inputs=8, outputs=4, ldx=8, ldy=4, low_rank_rows=1,
+                        d_x=4096, d_y=4096, d_plan=4096)
+    io.weight = _lib.Weights(4096, 32, 4, 1)
+    L = _lib.lib()
+    assert L.gn2v_typed_product(C.byref(io), None) == 1 and b"too many rows" in L.gn2v_last_error()
+    io.low_rank_rows, io.inputs, io.ldx, io.weight.inner = 0, 600, 600, 4
+    assert L.gn2v_typed_product(C.byref(io), None) == 1 and b"too many rows" in L.gn2v_last_error()
+
+
+# ------------------------------------------------------------------------------------ large sizes
+@pytest.mark.gpu
+def test_gradients_whose_join_fills_more_than_one_launch():
+    """16 types of 8 192 x 8 192: the sums of 2^30 weights are joined by more threads than a launch holds,
+    and types without rows get their zeros there."""
+    types, size = 16, 8192
+    gen = torch.Generator().manual_seed(0)
+    ids = torch.tensor([0, 3, 3, 15, -1, 9, 0, 3, 15, 15, 1, 16])
+    x, dy = (torch.randn(len(ids), size, generator=gen).bfloat16().cuda() for _ in range(2))
+    w = torch.zeros(1, 1, 1, dtype=torch.bfloat16, device="cuda").expand(types, size, size).contiguous().requires_grad_()
+    y = E.typed_projection(x, w, ids.cuda())
+    assert bool((y == 0).all())
+    (dw,) = torch.autograd.grad(y, w, dy)
+    for t in range(types):
+        at = (ids == t).nonzero().squeeze(1).cuda()
+        if not len(at):
+            assert bool((dw[t] == 0).all()), t
+            continue
+        a, b = x[at].double(), dy[at].double()
+        want, terms = a.T @ b, a.abs().T @ b.abs()
+        # a float32 sum of len(at) products, rounded to bfloat16
+        tolerance = (len(at) + 2) * 2.0 ** -24 * terms + 2.0 ** -8 * want.abs()
+        assert bool(((dw[t].double() - want).abs() <= tolerance).all()), t
