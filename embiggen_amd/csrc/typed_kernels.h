@@ -340,14 +340,16 @@ __device__ __forceinline__ u32x4 load_chunk(const T *row, int k, int length, int
 // nearest bfloat16 (ties to even; NaN stays NaN)
 __device__ __forceinline__ __bf16 to_bf16(float v) { return (__bf16)v; }
 
-// A float as two bfloat16 parts, 2^-16 of it left out at most: its upper half, and what that leaves,
-// rounded to nearest.  Both have its sign and neither is zero unless it is: an infinite factor makes the
-// same infinity of both parts, not a NaN.
+// A float as two bfloat16 parts: its upper half, and what that leaves, rounded to nearest (2^-16 of it left out
+// at most).  Where nothing is left, or less than a normal number, the parts are two halves of the upper half: both
+// have its sign and neither is zero, so that an infinite factor makes the same infinity of both, not a NaN, and
+// their sum is the value.  That holds from 2^-125 on, and the 2^-16 from 2^-110 on; below, 2^-126 of it is left out.
 __device__ __forceinline__ void split(float v, __bf16 &high, __bf16 &rest) {
-    const uint32_t bits = __float_as_uint(v) & 0xFFFF0000u;
-    high = __builtin_bit_cast(__bf16, (uint16_t)(bits >> 16));
-    const float left = v - __uint_as_float(bits);  // exact; NaN of an infinity
-    rest = to_bf16(__builtin_fabsf(left) > 0.f ? left : __builtin_copysignf(v != 0.f ? 0x1p-126f : 0.f, v));
+    const float upper = __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+    const float left = v - upper, half = 0.5f * upper;  // exact; `left` is NaN of an infinity
+    const bool both = __builtin_fabsf(left) >= 0x1p-126f;
+    high = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(both ? upper : half) >> 16));
+    rest = to_bf16(both ? left : half);
 }
 
 // four consecutive output elements, `valid` of them inside the row

@@ -97,3 +97,59 @@ def test_gradients_whose_join_fills_more_than_one_launch():
         # a float32 sum of len(at) products, rounded to bfloat16
         tolerance = (len(at) + 2) * 2.0 ** -24 * terms + 2.0 ** -8 * want.abs()
         assert bool(((dw[t].double() - want).abs() <= tolerance).all()), t
+
+
+# ------------------------------------------------------------- the two parts of a low-rank row (bfloat16)
+def same(got, want, what):
+    got = got.cpu()
+    assert got.shape == want.shape and got.dtype == want.dtype, what
+    other = (got != want).nonzero()  # NaN is another value
+    if len(other):
+        at = tuple(other[0].tolist())
+        raise AssertionError(f"{what}: {len(other)} of {got.numel()} differ, first {at}: {got[at]!r}, not {want[at]!r}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("inputs,rank", [(40, 5), (40, 20), (300, 5)])
+def test_small_low_rank_rows_keep_their_value(rows, inputs, rank):
+    """Low-rank rows of 2^-120 times weights, rows and gradients of 2^120: one, and no part of theirs added."""
+    ids = torch.arange(rows) % 3
+    outputs, small, large, dtype = 70, 2.0 ** -60, 2.0 ** 120, torch.bfloat16
+    counts = torch.bincount(ids).to(dtype)  # at most 100: exact
+    x, w, dy = torch.zeros(rows, inputs), torch.zeros(inputs, outputs), torch.zeros(rows, outputs)
+    down, up = torch.zeros(3, inputs, rank), torch.zeros(3, rank, outputs)
+    x[:, 0], down[:, 0, 0], up[:, 0], dy[:] = small, small, large, large
+    x, w, down, up, dy = (v.to(dtype).cuda() for v in (x, w, down, up, dy))
+    one = torch.ones(rows, outputs, dtype=dtype)
+    with torch.no_grad():
+        same(E.adapted_projection(x, w, down, up, ids.cuda()), one, "forward")
+    leaf = up.clone().requires_grad_()
+    y = E.adapted_projection(x, w, down, leaf, ids.cuda())
+    same(y.detach(), one, "y")
+    (d_up,) = torch.autograd.grad(y, leaf, dy)
+    same(d_up[:, 0], counts[:, None].expand(3, outputs), "d_up")
+    assert bool((d_up[:, 1:] == 0).all())
+    # the way back: dy up^T is 2^-120
+    x, down, up, dy = (torch.zeros_like(v) for v in (x, down, up, dy))
+    x[:], down[:, :, 0], up[:, 0, 0], dy[:, 0] = large, large, small, small
+    leaves = [v.requires_grad_() for v in (x, down)]
+    dx, d_down = torch.autograd.grad(E.adapted_projection(x, w, down, up, ids.cuda()), leaves, dy)
+    same(dx, torch.ones(rows, inputs, dtype=dtype), "dx")
+    same(d_down[:, :, 0], counts[:, None].expand(3, inputs), "d_down")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("inputs,rank", [(40, 5), (40, 20), (300, 5)])
+def test_small_low_rank_rows_times_infinity(rows, inputs, rank):
+    """Low-rank rows that take two parts, the second of them too small for a normal number."""
+    ids = torch.arange(rows) % 3
+    x, down = torch.zeros(rows, inputs), torch.zeros(3, inputs, rank)
+    x[:, 0], down[:, 0] = 2.0 ** -62 * (1 + 2.0 ** -7), 2.0 ** -60 * (1 + 2.0 ** -7)
+    up = torch.full((3, rank, 70), float("inf"))
+    x, w, down, up = (v.bfloat16().cuda() for v in (x, torch.zeros(inputs, 70), down, up))
+    with torch.no_grad():
+        assert bool((E.adapted_projection(x, w, down, up, ids.cuda()) == float("inf")).all())
+    y = E.adapted_projection(x, w, down.requires_grad_(), up, ids.cuda())
+    assert bool((y == float("inf")).all())
