@@ -99,7 +99,27 @@ def test_gradients_whose_join_fills_more_than_one_launch():
         assert bool(((dw[t].double() - want).abs() <= tolerance).all()), t
 
 
-# ------------------------------------------------------------- the two parts of a low-rank row (bfloat16)
+# ------------------------------------------------------------------- many tiles a workgroup, exactly
+# Rows, weights and gradients are small whole numbers and the scale is a power of two, so that every sum is
+# exact in float32, in any order (its terms' magnitudes add up to less than 2^24), and so are the two
+# bfloat16 parts of a low-rank row (whole numbers below 2^16, halved).  Results equal the definition in 64
+# bits, rounded once.
+def whole(gen, most, *shape):
+    return torch.randint(-most, most + 1, shape, generator=gen, dtype=torch.int8).double()
+
+
+def skewed_types(gen, rows, types):
+    """A few common types, a tail of rare ones and rows without a type."""
+    ids = (torch.rand(rows, generator=gen) ** 3 * types).long().clamp_(max=types - 1)
+    ids[torch.rand(rows, generator=gen) < 0.03] = -1
+    return ids
+
+
+def rounded(value, dtype):
+    assert float(value.abs().max()) < 2 ** 24
+    return value.float().to(dtype)
+
+
 def same(got, want, what):
     got = got.cpu()
     assert got.shape == want.shape and got.dtype == want.dtype, what
@@ -109,6 +129,109 @@ def same(got, want, what):
         raise AssertionError(f"{what}: {len(other)} of {got.numel()} differ, first {at}: {got[at]!r}, not {want[at]!r}")
 
 
+def exact_steps(x, ids, dy, weight=None, bias=None, shared=None, down=None, up=None, scale=0.5):
+    """Results and gradients in 64 bits: of the typed form (weight, bias by type) or of the adapted one
+    (shared, bias, down, up)."""
+    out = {}
+    if weight is not None:
+        out["y"], out["dx"] = x.new_zeros(len(x), weight.shape[2]), torch.zeros_like(x)
+        out["dw"], out["db"] = torch.zeros_like(weight), torch.zeros_like(bias)
+    else:
+        out["y"], out["dx"] = x @ shared + bias, dy @ shared.T
+        out["dw"], out["d_down"], out["d_up"] = x.T @ dy, torch.zeros_like(down), torch.zeros_like(up)
+        out["db"] = dy.sum(0)
+    for t in range(len(weight if weight is not None else down)):
+        at = (ids == t).nonzero().squeeze(1)
+        xt, dyt = x[at], dy[at]
+        if weight is not None:
+            out["y"][at], out["dx"][at] = xt @ weight[t] + bias[t], dyt @ weight[t].T
+            out["dw"][t], out["db"][t] = xt.T @ dyt, dyt.sum(0)
+        else:
+            low, back = scale * xt @ down[t], scale * dyt @ up[t].T
+            out["y"][at] += low @ up[t]
+            out["dx"][at] += back @ down[t].T
+            out["d_down"][t], out["d_up"][t] = xt.T @ back, low.T @ dyt
+    return out
+
+
+def run_steps(x, ids, dy, weight=None, bias=None, shared=None, down=None, up=None, scale=0.5):
+    if weight is not None:
+        leaves = [v.clone().requires_grad_() for v in (x, weight, bias)]
+        y = E.typed_projection(leaves[0], leaves[1], ids, bias=leaves[2])
+        names = ("dx", "dw", "db")
+    else:
+        leaves = [v.clone().requires_grad_() for v in (x, shared, down, up, bias)]
+        y = E.adapted_projection(*leaves[:4], ids, bias=leaves[4], scale=scale)
+        names = ("dx", "dw", "d_down", "d_up", "db")
+    return {"y": y.detach(), **dict(zip(names, torch.autograd.grad(y, leaves, dy)))}
+
+
+def check_steps(dtype, ids, **tensors):
+    want = exact_steps(ids=ids, **tensors)
+    plan = E.TypePlan(ids.cuda(), len(tensors["weight" if "weight" in tensors else "down"]))
+    device = {name: v.to(dtype).cuda() for name, v in tensors.items()}
+    got, again = run_steps(ids=plan, **device), run_steps(ids=ids.int().cuda(), **device)
+    for name, value in want.items():
+        same(got[name], rounded(value, dtype), name)
+        same(again[name], got[name].cpu(), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,types,inputs,outputs", [
+    # 3 438 tiles: seven a workgroup of the product, three of the gradients' 1 024
+    (220_001, 5, 16, 16), (150_003, 301, 90, 40), (130_001, 6, 100, 71), (140_000, 4, 128, 128), (100_001, 9, 192, 70),
+    # nine blocks of columns, 64 workgroups each
+    (15_001, 3, 40, 1100),
+    # longer rows: 141 tiles of gradients for 32 workgroups a block; outputs above the widest block of columns
+    (9_001, 4, 512, 512), (700, 3, 300, 257), (1_400, 5, 520, 390), (2_000, 1, 260, 150)])
+def test_typed_steps_of_many_tiles(rows, types, inputs, outputs, dtype):
+    gen = torch.Generator().manual_seed(rows + outputs)
+    ids = skewed_types(gen, rows, types)
+    check_steps(dtype, ids, x=whole(gen, 2, rows, inputs), dy=whole(gen, 2, rows, outputs),
+                weight=whole(gen, 3, types, inputs, outputs), bias=whole(gen, 5, types, outputs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,types,inputs,outputs,rank", [
+    # 2 500 tiles: five a workgroup of the products, three to five of the gradients
+    (160_001, 5, 16, 16, 3), (150_003, 237, 64, 40, 8), (110_001, 5, 128, 128, 16), (110_001, 7, 100, 33, 5),
+    (100_001, 4, 256, 30, 16), (12_001, 3, 64, 1100, 4),
+    # longer rows or ranks
+    (20_001, 6, 300, 40, 20), (1_400, 4, 520, 390, 16), (1_200, 100, 260, 150, 40), (60_001, 5, 40, 48, 33)])
+def test_adapted_steps_of_many_tiles(rows, types, inputs, outputs, rank, dtype):
+    gen = torch.Generator().manual_seed(rows + outputs)
+    ids = skewed_types(gen, rows, types)
+    check_steps(dtype, ids, x=whole(gen, 1, rows, inputs), dy=whole(gen, 1, rows, outputs),
+                shared=whole(gen, 3, inputs, outputs), bias=whole(gen, 5, outputs),
+                down=whole(gen, 1, types, inputs, rank), up=whole(gen, 1, types, rank, outputs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_frozen_and_single_gradients_of_many_tiles(dtype):
+    """The corrections alone (one pass over the rows without the shared weight's sums), and each gradient by itself."""
+    gen = torch.Generator().manual_seed(3)
+    rows, types, inputs, outputs, rank = 120_001, 40, 100, 96, 5
+    ids = skewed_types(gen, rows, types)
+    tensors = dict(x=whole(gen, 1, rows, inputs), dy=whole(gen, 1, rows, outputs), shared=whole(gen, 3, inputs, outputs),
+                   bias=whole(gen, 5, outputs), down=whole(gen, 1, types, inputs, rank),
+                   up=whole(gen, 1, types, rank, outputs))
+    want = {name: rounded(v, dtype) for name, v in exact_steps(ids=ids, **tensors).items()}
+    device = {name: v.to(dtype).cuda() for name, v in tensors.items()}
+    plan = E.TypePlan(ids.cuda(), types)
+    order = ["x", "shared", "down", "up", "bias"]
+    gradients = dict(zip(order, ("dx", "dw", "d_down", "d_up", "db")))
+    for wanted in (["x", "down", "up"], ["down", "up"], ["x"], ["down"], ["up"], ["shared"], ["bias"], ["down", "up", "bias"]):
+        leaves = {name: device[name].clone().requires_grad_(name in wanted) for name in order}
+        y = E.adapted_projection(*(leaves[name] for name in order[:4]), plan, bias=leaves["bias"], scale=0.5)
+        same(y.detach(), want["y"], "y")
+        for name, got in zip(wanted, torch.autograd.grad(y, [leaves[name] for name in wanted], device["dy"])):
+            same(got, want[gradients[name]], (wanted, name))
+
+
+# ------------------------------------------------------------- the two parts of a low-rank row (bfloat16)
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [20, 300])
 @pytest.mark.parametrize("inputs,rank", [(40, 5), (40, 20), (300, 5)])
@@ -153,3 +276,66 @@ def test_small_low_rank_rows_times_infinity(rows, inputs, rank):
         assert bool((E.adapted_projection(x, w, down, up, ids.cuda()) == float("inf")).all())
     y = E.adapted_projection(x, w, down.requires_grad_(), up, ids.cuda())
     assert bool((y == float("inf")).all())
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows whose elements, read and written, lie more than 2^31 elements and 2^32 bytes behind the first; the sums of
+    a type's millions of rows stay below 2^24."""
+    rows, types, inputs, outputs, dtype = 17_000_000, 5, 24, 136, torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(0)
+
+    def draw(most, *shape):
+        return torch.randint(-most, most + 1, shape, generator=gen, dtype=torch.int8, device="cuda").to(dtype)
+
+    x = torch.zeros(rows, 128, dtype=dtype, device="cuda")[:, :inputs]  # rows of a padded table
+    x.copy_(draw(1, rows, inputs))
+    dy = draw(1, rows, outputs)
+    w, b = draw(2, types, inputs, outputs), draw(3, types, outputs)
+    ids = torch.randint(-1, types, (rows,), generator=gen, dtype=torch.int32, device="cuda")
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    y = E.typed_projection(leaves[0], leaves[1], ids, bias=leaves[2])
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    y = y.detach()
+    for t in range(-1, types):
+        at = (ids == t).nonzero().squeeze(1)
+        if t < 0:
+            assert bool((y[at] == 0).all()) and bool((dx[at] == 0).all())
+            continue
+        sums = torch.zeros(inputs, outputs, dtype=torch.float64, device="cuda")
+        for part in at.split(1 << 20):
+            xt, dyt = x[part].double(), dy[part].double()
+            assert torch.equal(y[part], rounded(xt @ w[t].double() + b[t].double(), dtype)), t
+            assert torch.equal(dx[part], rounded(dyt @ w[t].double().T, dtype)), t
+            sums += xt.T @ dyt
+        assert torch.equal(dw[t], rounded(sums, dtype)), t
+        assert torch.equal(db[t], rounded(dy[at].double().sum(0), dtype)), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [700, 40_000])
+def test_forward_and_backward_on_a_side_stream(rows):
+    gen = torch.Generator().manual_seed(1)
+    ids = skewed_types(gen, rows, 6)
+    tensors = dict(x=whole(gen, 1, rows, 64), dy=whole(gen, 1, rows, 48), shared=whole(gen, 3, 64, 48),
+                   bias=whole(gen, 5, 48), down=whole(gen, 1, 6, 64, 4), up=whole(gen, 1, 6, 4, 48))
+    want = exact_steps(ids=ids, **tensors)
+    device = {name: v.float().cuda() for name, v in tensors.items()}
+    types = ids.cuda()
+    here = run_steps(ids=types, **device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = run_steps(ids=types, **device)
+    # forward on the side stream, backward called from this one: it runs where the forward did
+    with torch.cuda.stream(side):
+        x = device["x"].clone().requires_grad_()
+        y = E.adapted_projection(x, device["shared"], device["down"], device["up"], types, bias=device["bias"], scale=0.5)
+    torch.cuda.current_stream().wait_stream(side)
+    (dx,) = torch.autograd.grad(y, x, device["dy"])
+    torch.cuda.synchronize()
+    for name, value in want.items():
+        same(here[name], rounded(value, torch.float32), name)
+        same(there[name], here[name].cpu(), name)
+    same(dx, here["dx"].cpu(), "dx")
+    same(y.detach(), here["y"].cpu(), "y")
