@@ -95,6 +95,10 @@ class QuantizedTable:
         self._io = _lib.Table8(codes.data_ptr(), scales.data_ptr(), codes.shape[0], size,
                                codes.shape[1], group_size, _codes()[codes.dtype])
 
+    def __reduce__(self):
+        # copies and pickles hold the tensors; the addresses are taken anew, behind the same checks
+        return type(self), (self._codes, self._scales, self.embedding_size, self.group_size)
+
     @classmethod
     def empty(cls, number_of_rows: int, embedding_size: int, dtype=None, group_size: int = 64,
               device: int = 0) -> "QuantizedTable":

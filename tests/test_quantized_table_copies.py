@@ -1,0 +1,52 @@
+"""8-bit tables as objects: copied, stored and taken up again, and where they are refused."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+import embiggen_amd as E
+from embiggen_amd import _lib
+
+
+def on_the_cpu(rows=4, width=20):
+    """A table that no device holds (the class refuses to make one)."""
+    table = E.QuantizedTable.__new__(E.QuantizedTable)
+    table._codes, table._scales = torch.zeros(rows, 32, dtype=torch.int8), torch.zeros(rows, 1)
+    table.embedding_size, table.group_size = width, 64
+    table._io = _lib.Table8(table._codes.data_ptr(), table._scales.data_ptr(), rows, width, 32, 64, 0)
+    return table
+
+
+def test_a_table_is_stored_by_its_tensors_and_checked_when_it_is_taken_up():
+    table = on_the_cpu()
+    stored = pickle.dumps(table)
+    for again in (lambda: pickle.loads(stored), lambda: copy.copy(table), lambda: copy.deepcopy(table)):
+        with pytest.raises(ValueError, match="no CPU execution path"):
+            again()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+def test_copies_of_a_table_and_of_a_transformer(codes):
+    gen = torch.Generator().manual_seed(0)
+    table = E.QuantizedTable.from_table(torch.randn(30, 37, generator=gen).cuda(), codes, 16)
+    values = table.read()
+    transformer = E.EdgeTransformer(["Hadamard", "CosineSimilarity"]).fit(table)
+    ids = torch.arange(30, device="cuda")
+    features = transformer.transform(ids, ids.flip(0))
+    file = io.BytesIO()
+    torch.save(table, file)
+    file.seek(0)
+    deep = [copy.deepcopy(table), pickle.loads(pickle.dumps(table)), torch.load(file, weights_only=False)]
+    shared = copy.copy(table)
+    transformers = [copy.deepcopy(transformer), pickle.loads(pickle.dumps(transformer))]
+    assert shared.codes is table.codes and shared.scales is table.scales
+    table.write(torch.zeros(30, 37).cuda())
+    for other in deep:
+        assert other.codes.dtype == codes and (other.shape, other.group_size) == (table.shape, 16)
+        assert torch.equal(other.read(), values)
+    for other in transformers:
+        assert torch.equal(other.transform(ids, ids.flip(0)), features)
+    assert bool((shared.read() == 0).all())
