@@ -11,6 +11,7 @@ import numpy as np
 
 from .edge_transformer import EdgeTransformer
 from .node_transformer import is_graph
+from .quantized_table import QuantizedTable
 
 
 class GraphTransformer:
@@ -21,6 +22,11 @@ class GraphTransformer:
         self._aligned_mapping = aligned_mapping
 
     def fit(self, node_feature, node_type_feature=None, edge_type_features=None):
+        features = node_feature if isinstance(node_feature, (list, tuple)) else [node_feature]
+        if any(isinstance(feature, QuantizedTable) for feature in features):
+            raise ValueError(
+                "The edges of a graph are embedded from arrays and DataFrames on the host: a table in 8 bits is "
+                "read by `EdgeTransformer` and `edge_embedding`, which take tensors of node ids.")
         self._transformer.fit(node_feature=node_feature, node_type_feature=node_type_feature,
                               edge_type_features=edge_type_features)
         return self

@@ -27,6 +27,19 @@ def test_a_table_is_stored_by_its_tensors_and_checked_when_it_is_taken_up():
             again()
 
 
+@pytest.mark.parametrize("transformer", [E.GraphTransformer, E.EdgePredictionTransformer, E.EdgeLabelPredictionTransformer])
+def test_transformers_of_graphs_refuse_a_table(transformer):
+    for features in (on_the_cpu(), [on_the_cpu()], (on_the_cpu(), on_the_cpu())):
+        with pytest.raises(ValueError, match="8 bits"):
+            transformer("Hadamard", aligned_mapping=True).fit(features)
+
+
+@pytest.mark.parametrize("transformer", [E.NodeTransformer, E.NodeLabelPredictionTransformer])
+def test_transformers_of_nodes_refuse_a_table(transformer):
+    with pytest.raises(ValueError, match="neither a pandas DataFrame nor a numpy array"):
+        transformer(aligned_mapping=True).fit(on_the_cpu())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
 def test_copies_of_a_table_and_of_a_transformer(codes):
