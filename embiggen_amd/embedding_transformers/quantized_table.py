@@ -94,6 +94,18 @@ class QuantizedTable:
         self.embedding_size, self.group_size = size, group_size
         self._io = _lib.Table8(codes.data_ptr(), scales.data_ptr(), codes.shape[0], size,
                                codes.shape[1], group_size, _codes()[codes.dtype])
+        self._taken = self._where()
+
+    def _where(self):
+        codes, scales = self._codes, self._scales
+        return codes.data_ptr(), scales.data_ptr(), codes.shape, scales.shape
+
+    def _table(self):
+        """The table for a call.  The tensors are the caller's too: one that has other memory now (its ``data`` set,
+        resized) is taken up anew, behind the same checks."""
+        if self._where() != self._taken:
+            self.__init__(self._codes, self._scales, self.embedding_size, self.group_size)
+        return self._io
 
     def __reduce__(self):
         # copies and pickles hold the tensors; the addresses are taken anew, behind the same checks
@@ -182,6 +194,7 @@ class QuantizedTable:
             rows = _ids(rows, values.device, "rows")
             if rows.shape[0] != n:
                 raise ValueError(f"There are {n} values, but rows for {rows.numel()}.")
+        io = self._table()
         apart, inner = values.stride()
         if inner != 1 or apart < self.embedding_size:
             values = values.detach().contiguous()
@@ -190,7 +203,7 @@ class QuantizedTable:
         if rows is not None and n > _lib.TABLE_FEW_ENTRIES:
             owner = torch.empty(len(self), dtype=torch.int32, device=self.device)
         _lib.check(_lib.lib().gn2v_table_write(
-            self._io, values.data_ptr(), kind, max(apart, self.embedding_size),
+            io, values.data_ptr(), kind, max(apart, self.embedding_size),
             None if rows is None else rows.data_ptr(), 0 if rows is None else rows.element_size(), n,
             None if owner is None else owner.data_ptr(), _stream(self._codes)))
 
@@ -205,7 +218,7 @@ class QuantizedTable:
         n = len(self) if rows is None else rows.shape[0]
         out = torch.empty((n, self.embedding_size), dtype=dtype, device=self._codes.device)
         _lib.check(_lib.lib().gn2v_table_read(
-            self._io, None if rows is None else rows.data_ptr(),
+            self._table(), None if rows is None else rows.data_ptr(),
             0 if rows is None else rows.element_size(), n, out.data_ptr(), kind,
             self.embedding_size, _stream(self._codes)))
         return out
@@ -230,6 +243,6 @@ def quantized_edge_embedding(table, sources, destinations, method: int, width: i
         src, dst = src.long(), dst.long()
     out = torch.empty((src.numel(), width), dtype=torch.float32, device=table.device)
     _lib.check(_lib.lib().gn2v_table_edge_embedding(
-        table._io, other._io, src.data_ptr(), dst.data_ptr(), src.element_size(),
+        table._table(), other._table(), src.data_ptr(), dst.data_ptr(), src.element_size(),
         src.numel(), method, out.data_ptr(), width, _stream(table.codes)))
     return out

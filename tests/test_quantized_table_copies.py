@@ -16,6 +16,7 @@ def on_the_cpu(rows=4, width=20):
     table._codes, table._scales = torch.zeros(rows, 32, dtype=torch.int8), torch.zeros(rows, 1)
     table.embedding_size, table.group_size = width, 64
     table._io = _lib.Table8(table._codes.data_ptr(), table._scales.data_ptr(), rows, width, 32, 64, 0)
+    table._taken = table._where()
     return table
 
 
@@ -25,6 +26,18 @@ def test_a_table_is_stored_by_its_tensors_and_checked_when_it_is_taken_up():
     for again in (lambda: pickle.loads(stored), lambda: copy.copy(table), lambda: copy.deepcopy(table)):
         with pytest.raises(ValueError, match="no CPU execution path"):
             again()
+
+
+def test_tensors_that_moved_are_checked_again():
+    table = on_the_cpu()
+    assert table._table() is table._io
+    for change in (lambda: setattr(table.codes, "data", torch.zeros(4, 32, dtype=torch.int8)),
+                   lambda: setattr(table.scales, "data", torch.zeros(4, 1)),
+                   lambda: table.codes.resize_(2, 32)):
+        change()
+        with pytest.raises(ValueError, match="no CPU execution path|The scales should be"):
+            table._table()
+        table._taken = table._where()
 
 
 @pytest.mark.parametrize("transformer", [E.GraphTransformer, E.EdgePredictionTransformer, E.EdgeLabelPredictionTransformer])
@@ -63,3 +76,19 @@ def test_copies_of_a_table_and_of_a_transformer(codes):
     for other in transformers:
         assert torch.equal(other.transform(ids, ids.flip(0)), features)
     assert bool((shared.read() == 0).all())
+
+
+@pytest.mark.gpu
+def test_tensors_that_moved_are_the_table():
+    gen = torch.Generator().manual_seed(0)
+    table, other = (E.QuantizedTable.from_table(torch.randn(n, 40, generator=gen).cuda(), group_size=16) for n in (30, 12))
+    want, ids = other.read(), torch.arange(30, device="cuda")
+    table.codes.data, table.scales.data = other.codes.clone(), other.scales.clone()
+    got = table.read(ids)
+    assert table.shape == (12, 40) and torch.equal(got[:12], want) and bool((got[12:] == 0).all())
+    table.write(torch.zeros(30, 40).cuda(), ids)  # the rows behind the last one are left out
+    assert bool((table.read() == 0).all()) and torch.equal(other.read(), want)
+    table.scales.data = other.scales[:5].clone()
+    for call in (table.read, lambda: table.write(want), lambda: E.edge_embedding(other, ids, ids, destination_table=table)):
+        with pytest.raises(ValueError, match="The scales should be"):
+            call()
