@@ -43,6 +43,10 @@ def _value_type(dtype) -> int:
     raise ValueError(f"Rows are float32 or bfloat16, but we got {dtype} instead.")
 
 
+def _taken_up(cls, codes, dtype, *rest):
+    return cls(codes.view(dtype), *rest)
+
+
 class QuantizedTable:
     """A table of ``embedding_size`` columns in 8 bits.
 
@@ -107,9 +111,14 @@ class QuantizedTable:
             self.__init__(self._codes, self._scales, self.embedding_size, self.group_size)
         return self._io
 
+    # Copies and pickles hold the tensors; the addresses are taken anew, behind the same checks.  Codes go as bytes:
+    # a tensor of float8 elements cannot be pickled by itself.
+    def __copy__(self):
+        return type(self)(self._codes, self._scales, self.embedding_size, self.group_size)
+
     def __reduce__(self):
-        # copies and pickles hold the tensors; the addresses are taken anew, behind the same checks
-        return type(self), (self._codes, self._scales, self.embedding_size, self.group_size)
+        return _taken_up, (type(self), self._codes.view(_torch().uint8), self._codes.dtype, self._scales,
+                           self.embedding_size, self.group_size)
 
     @classmethod
     def empty(cls, number_of_rows: int, embedding_size: int, dtype=None, group_size: int = 64,
