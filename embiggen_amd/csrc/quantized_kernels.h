@@ -412,9 +412,11 @@ __global__ __launch_bounds__(256) void table_scores_kernel(TableView src, TableV
                 if constexpr (METHOD == kCosineSimilarity) {
                     float x, y, z;
                     dot16<CODE>(p[u].code, q[u].code, x, y, z);
-                    ab[u] = fmaf(x, p[u].scale * q[u].scale, ab[u]);
-                    aa[u] = fmaf(y, p[u].scale * p[u].scale, aa[u]);
-                    bb[u] = fmaf(z, q[u].scale * q[u].scale, bb[u]);
+                    // one scale after the other, the smaller one first: the product of two may pass float32's
+                    // largest number where the codes are zero (a NaN scale still reaches aa or bb)
+                    ab[u] = fmaf(x * fminf(p[u].scale, q[u].scale), fmaxf(p[u].scale, q[u].scale), ab[u]);
+                    aa[u] = fmaf(y * p[u].scale, p[u].scale, aa[u]);
+                    bb[u] = fmaf(z * q[u].scale, q[u].scale, bb[u]);
                 } else {
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
