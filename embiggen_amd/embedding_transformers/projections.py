@@ -98,7 +98,6 @@ class TypePlan:
         _check_device(types)
         self.number_of_types = int(number_of_types)
         self.number_of_rows = types.numel()
-        self.device = types.device
         words, temp_words = _plan_words(self.number_of_rows, self.number_of_types)
         types = types.contiguous()
         self._words = torch.empty(words, dtype=torch.int32, device=types.device)
@@ -123,6 +122,10 @@ class TypePlan:
         ids = np.ascontiguousarray(ids, dtype=np.uint32).view(np.int32)
         count = max(1, int(ids.max(initial=-1)) + 1)
         return cls(_torch().from_numpy(ids).to(_torch().device("cuda", device)), count)
+
+    @property
+    def device(self):
+        return self._words.device
 
     @property
     def order(self):

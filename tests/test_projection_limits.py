@@ -62,6 +62,18 @@ def test_forward_mode_derivatives_are_refused(on_the_cpu, rows):
             twice[0].sum().backward()
 
 
+def test_a_plan_is_where_its_words_are(on_the_cpu):
+    """A stored plan may be loaded onto another device than it was made on."""
+    plan = E.TypePlan(torch.tensor([0, 1, -1]), 2)
+    x, w = torch.zeros(3, 4), torch.zeros(2, 4, 5)
+    assert E.typed_projection(x, w, plan).shape == (3, 5)
+    plan._words = plan._words.to("meta")
+    with pytest.raises(ValueError, match="types are on meta"):
+        E.typed_projection(x, w, plan)
+    with pytest.raises(ValueError, match="types are on meta"):
+        E.adapted_projection(x, w[0], torch.zeros(2, 4, 1), torch.zeros(2, 1, 5), plan)
+
+
 def test_launches_of_too_many_threads_are_refused():
     """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256, one per 64 rows of the low-rank rows."""
     rows = (1 << 30) + (1 << 20)
