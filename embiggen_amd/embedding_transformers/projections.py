@@ -14,7 +14,7 @@ import collections
 import ctypes as C
 import functools
 import struct
-from typing import Optional, Union
+from typing import Union
 
 from .. import _lib
 
@@ -439,6 +439,15 @@ def _check_types(types, x, number_of_types: int):
         raise ValueError(f"The types are on {device}, but the rows on {x.device}.")
 
 
+def _check_scale(scale) -> float:
+    if getattr(scale, "requires_grad", False):
+        raise ValueError("The provided scale takes no gradient: multiply `up` by it instead.")
+    try:
+        return float(scale)
+    except (TypeError, ValueError, RuntimeError):
+        raise ValueError(f"The provided scale should be a number, but we got {scale!r} instead.") from None
+
+
 def _refuse_tangents(*tensors):
     """The kernels see a tensor's values alone: a forward-mode tangent would be lost without a word."""
     forward_ad = _torch().autograd.forward_ad
@@ -498,7 +507,7 @@ def typed_projection(x, weight, types: Union["TypePlan", "object"], bias=None):
 
 
 def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], bias=None,
-                       scale: Optional[float] = 1.0):
+                       scale: float = 1.0):
     """``x[r] @ weight + bias + scale * (x[r] @ down[types[r]]) @ up[types[r]]`` for every row: one
     projection that all rows share and a low-rank correction of their type.  Rows of unknown type get
     the shared part alone.
@@ -516,7 +525,7 @@ def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], 
     bias
         [outputs] or None.
     scale: float
-        Of the correction.
+        Of the correction; a number, which takes no gradient.
 
     Returns
     ------------------
@@ -544,7 +553,7 @@ def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], 
     _check_device(x)
     _refuse_tangents(x, weight, down, up, bias)
     plan = types if isinstance(types, TypePlan) else None
-    scale = float(scale)
+    scale = _check_scale(scale)
     if not _wants_gradient(x, weight, down, up, bias):
         y = _few_rows(x, plan, types, weight, n_types, bias, down, up, scale)
         if y is not None:

@@ -2,6 +2,7 @@
 derivatives, many tiles a workgroup, sizes that pass 32 bits, other streams."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -72,6 +73,15 @@ def test_a_plan_is_where_its_words_are(on_the_cpu):
         E.typed_projection(x, w, plan)
     with pytest.raises(ValueError, match="types are on meta"):
         E.adapted_projection(x, w[0], torch.zeros(2, 4, 1), torch.zeros(2, 1, 5), plan)
+
+
+def test_scales_that_are_no_numbers_are_refused(on_the_cpu):
+    tensors = [torch.zeros(3, 4), torch.zeros(4, 5), torch.zeros(2, 4, 1), torch.zeros(2, 1, 5), torch.tensor([0, 1, -1])]
+    for scale in (None, "half", torch.ones(2), torch.tensor(0.5, requires_grad=True)):
+        with pytest.raises(ValueError, match="scale"):
+            E.adapted_projection(*tensors, scale=scale)
+    for scale in (2, 0.5, torch.tensor(0.5), np.float64(0.25)):
+        assert E.adapted_projection(*tensors, scale=scale).shape == (3, 5)
 
 
 def test_launches_of_too_many_threads_are_refused():
