@@ -774,7 +774,7 @@ __global__ __launch_bounds__(kNarrowThreads, 4) void narrow_product_kernel(Produ
     constexpr int FIT = LDS_W / (WT ? BN * (SLAB + Tile<T>::kPad) : SLAB * WS);
     constexpr int STEP = narrow_step(SLABS, FIT);
     constexpr int WTS = STEP * SLAB + Tile<T>::kPad;
-    static_assert((WT ? BN * WTS : STEP * SLAB * WS) <= LDS_W || STEP == 1, "weights in passes");
+    static_assert((WT ? BN * WTS : STEP * SLAB * WS) <= LDS_W, "weights in passes");
     __shared__ __align__(16) T xs[LDS_W];
     __shared__ __align__(16) T ls[ADAPT ? ROWS * LS : 1];
     __shared__ __align__(16) T as[ADAPT ? 16 * XS : 1];

@@ -6,9 +6,9 @@ an adapter.  The reference's classifiers treat types as one-hot columns beside t
 (embiggen/embedding_transformers/graph_transformer.py:196-243); here every type has weights of its own.
 Both run in hand-written kernels that read the rows where they are: a *plan* (``TypePlan``) holds the
 order of the rows by type, and no sorted copy of them is made.  Both can be differentiated backwards, once
-(forward-mode derivatives are refused); gradients are summed in a fixed order, so a run gives the same bits every time.  Calls are made on the current
-stream and can be captured into a graph, the plan's among them; a backward pass that is captured takes
-leaves that no eager graph holds at the time.
+(forward-mode derivatives are refused); gradients are summed in a fixed order, so a run gives the same bits
+every time.  Calls are made on the current stream and can be captured into a graph, the plan's among them; a
+backward pass that is captured takes leaves that no eager graph holds at the time.
 """
 import collections
 import ctypes as C
@@ -293,6 +293,7 @@ def _adapted_gradient(x, dy, low, back, rank, plan, d_down, d_up, dw, db):
 # (the plan given), microseconds: 128 -> 128 float32, 1 024 rows 6.4 / 20.5 (10.2), 4 096 rows 16.6 / 22.4
 # (11.7); 512 -> 256, 512 rows (268 MB) float32 15.7 / 44.4 (34.9), 1 024 rows bfloat16 (268 MB) 18.3 /
 # 23.6 (13.6), 2 048 rows (537 MB) 32.4 / 23.2 (13.7); 1 024 -> 1 024, 64 rows (268 MB) float32 18.1 / 68.4.
+# One rule, plan or none: with a plan at hand the largest bfloat16 calls inside it lose up to 5 us.
 FEW_ROWS = 1024
 FEW_BYTES = 1 << 28
 

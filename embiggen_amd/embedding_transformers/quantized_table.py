@@ -51,8 +51,9 @@ class QuantizedTable:
     """A table of ``embedding_size`` columns in 8 bits.
 
     The scale of a group is its largest magnitude times the float32 1 / 127 (int8) or 1 / 448 (e4m3), in
-    float32, and at least 2**-90; a code is the value divided by it, rounded to the nearest code, ties to even; a value read back is
-    code * scale.  A group that holds an infinity or a NaN reads back as NaN.
+    float32 (within 2**-23 of the quotient), and at least 2**-90; a code is the value divided by it, rounded to
+    the nearest code, ties to even; a value read back is code * scale.  A group that holds an infinity or a NaN
+    reads back as NaN.
 
     Parameters
     ------------------
