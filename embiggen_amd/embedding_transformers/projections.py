@@ -85,6 +85,8 @@ class TypePlan:
         ``[0, number_of_types)`` -- is an unknown type.
     number_of_types: int
         How many types there are, 32 768 at most.
+
+    A plan may be used on other streams than the one that it was made on, once they wait for it.
     """
 
     def __init__(self, types, number_of_types: int):
@@ -100,13 +102,24 @@ class TypePlan:
         self.number_of_rows = types.numel()
         words, temp_words = _plan_words(self.number_of_rows, self.number_of_types)
         types = types.contiguous()
+        self._made_on = _stream(types)
         self._words = torch.empty(words, dtype=torch.int32, device=types.device)
         temp = None
         if temp_words:
             temp = torch.empty(temp_words, dtype=torch.int32, device=types.device)
         _lib.check(_lib.lib().gn2v_type_plan(
             types.data_ptr(), types.element_size(), self.number_of_rows, self.number_of_types,
-            self._words.data_ptr(), None if temp is None else temp.data_ptr(), _stream(types)))
+            self._words.data_ptr(), None if temp is None else temp.data_ptr(), self._made_on))
+
+    def _used_by(self, x):
+        """Called before a projection of ``x``: the words are row ids that kernels follow, so their memory is not given
+        to others while another stream than the plan's still reads them."""
+        if _stream(x) != self._made_on:
+            self._words.record_stream(_torch().cuda.current_stream(x.device))
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._made_on = None  # a copy's words are of another stream, or of another process
 
     @classmethod
     def from_graph(cls, graph, of: str = "nodes", device: int = 0) -> "TypePlan":
@@ -500,6 +513,8 @@ def typed_projection(x, weight, types: Union["TypePlan", "object"], bias=None):
     _check_device(x)
     _refuse_tangents(x, weight, bias)
     plan = types if isinstance(types, TypePlan) else None
+    if plan is not None:
+        plan._used_by(x)
     if not _wants_gradient(x, weight, bias):
         y = _few_rows(x, plan, types, weight, n_types, bias)
         if y is not None:
@@ -554,6 +569,8 @@ def adapted_projection(x, weight, down, up, types: Union["TypePlan", "object"], 
     _check_device(x)
     _refuse_tangents(x, weight, down, up, bias)
     plan = types if isinstance(types, TypePlan) else None
+    if plan is not None:
+        plan._used_by(x)
     scale = _check_scale(scale)
     if not _wants_gradient(x, weight, down, up, bias):
         y = _few_rows(x, plan, types, weight, n_types, bias, down, up, scale)

@@ -1,6 +1,8 @@
 """What the projections refuse, and how they behave at the ends of what they allow: forward-mode
 derivatives, many tiles a workgroup, sizes that pass 32 bits, other streams."""
+import copy
 import ctypes as C
+import pickle
 
 import numpy as np
 import pytest
@@ -361,3 +363,68 @@ def test_forward_and_backward_on_a_side_stream(rows):
         same(there[name], here[name].cpu(), name)
     same(dx, here["dx"].cpu(), "dx")
     same(y.detach(), here["y"].cpu(), "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [700, 40_000])
+def test_the_memory_of_a_plan_waits_for_the_streams_that_read_it(rows):
+    """A plan that goes out of scope while another stream has yet to use it: its words are row ids, and whoever gets
+    their memory would send the kernels anywhere."""
+    gen = torch.Generator().manual_seed(2)
+    ids = skewed_types(gen, rows, 6)
+    x, w = whole(gen, 1, rows, 64).float().cuda(), whole(gen, 2, 6, 64, 48).float().cuda()
+    want = E.typed_projection(x, w, ids.cuda())
+    a = torch.zeros(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+    plan = E.TypePlan(ids.cuda(), 6)
+    words, at = plan._words.numel(), plan._words.data_ptr()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(40):  # some 40 ms of work before the projection
+            a = a @ a
+        y = E.typed_projection(x, w, plan)
+    del plan
+    others = [torch.empty(words, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not side.query(), "the side stream is still at work"
+    assert at not in [other.data_ptr() for other in others]
+    side.synchronize()
+    same(y, want.cpu(), "y")
+    # a copy's words lie elsewhere, whatever stream is the current one
+    plan = E.TypePlan(ids.cuda(), 6)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        again = [copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))]
+        side.synchronize()
+    for other in again:
+        assert torch.equal(other.order, plan.order) and torch.equal(other.offsets, plan.offsets)
+        same(E.typed_projection(x, w, other), want.cpu(), "copy")
+
+
+@pytest.mark.gpu
+def test_steps_captured_around_a_plan_made_before():
+    gen = torch.Generator().manual_seed(4)
+    rows, types = 3_000, 6
+    ids = skewed_types(gen, rows, types)
+    plan = E.TypePlan(ids.cuda(), types)
+    draw = lambda: dict(x=whole(gen, 1, rows, 64), dy=whole(gen, 1, rows, 48), shared=whole(gen, 3, 64, 48),  # noqa: E731
+                        bias=whole(gen, 5, 48), down=whole(gen, 1, types, 64, 4), up=whole(gen, 1, types, 4, 48))
+    state = {name: v.float().cuda() for name, v in draw().items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run_steps(ids=plan, **state)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run_steps(ids=plan, **state)
+    for _ in range(3):
+        tensors = draw()
+        for name, v in tensors.items():
+            state[name].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, value in exact_steps(ids=ids, **tensors).items():
+            same(captured[name], rounded(value, torch.float32), name)
+    del plan, graph
+    torch.cuda.synchronize()
+    same(E.TypePlan(ids.cuda(), types).order, torch.argsort(torch.where(ids < 0, types, ids), stable=True).int(), "order")
